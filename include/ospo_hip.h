@@ -533,6 +533,57 @@ int ospo_decode_attn_o(const void* q, int ldq, const void* k_cache, const void* 
                        const void* residual, int ldr, void* out, int ldo, float* ss_out, const int* step_dev,
                        int layer, unsigned* flags, unsigned* tmo, void* ws, size_t ws_bytes, hipStream_t stream);
 
+/* ------------------------------------------------------------ paged cache ---
+ * Serving over a cache of pages: unlike lengths side by side, grouped heads, long contexts.  bf16 (dtype 0) or fp16
+ * (dtype 1), the rotation also fp32 (dtype 2).  Strides are in ELEMENTS; the last dimension is contiguous.
+ *
+ * A batch is ragged: the rows (new tokens) of sequence s are q_start[s] .. q_start[s + 1] - 1 (int32 [n_seqs + 1],
+ * not descending), kv_len[s] (int32) is its length WITH them, so row r sits at position
+ * kv_len[s] - q_start[s + 1] + r.  Position p lives in page block_table[s][p / page_size] (int32
+ * [n_seqs][max_pages]), slot p % page_size; page_size >= 1 is any number, max_pages * page_size < 2^31.  A cache
+ * tensor is [n_pages][kv heads][page_size][head_dim] by page_stride, head_stride and slot_stride.  All of these
+ * are read on the device: a captured call follows their values at each replay.  Values outside their range cannot
+ * fault: row numbers and lengths are clamped to the buffers, a page outside [0, n_pages) is not written by the
+ * append and read as the nearest page by the attention.  Rows of no sequence are left as they were.
+ *
+ * ospo_rotary: rotary positions on q (and k, n_k_heads = 0: none), out of place or in place (equal pointers and
+ *   strides; buffers that overlap otherwise are not supported).  Of each head the first rot_dim elements (even)
+ *   turn, in pairs (i, i + rot_dim / 2), or (2i, 2i + 1) with interleaved = 1; the rest is copied.
+ *     y1 = x1 c - x2 s,  y2 = x2 c + x1 s      c, s = cos_tab, sin_tab [min(positions[r], n_pos - 1)][i] (fp32)
+ *   in fp32, rounded once.  backward = 1: the gradient (sin negated): dx from dy, for the tables as they are
+ *   (a magnitude in them scales both directions).  positions: int32 [n], clamped to [0, n_pos).  head_dim <= 256.
+ *   Any strides and alignment; 16-byte accesses where they allow it.
+ * ospo_paged_append: k (turned by the tables' row of its position, rot_dim = 0: as it is) and v of every row into
+ *   the caches, q turned into q_out (n_q_heads = 0: none).  Same arithmetic as ospo_rotary.  A row whose position
+ *   is negative, past max_pages * page_size, or in a page outside [0, n_pages) is not stored (its q_out is written).
+ *   Two rows that land on the same slot: either one's values.
+ * ospo_paged_attn: out[r][h] = softmax(scale q[r][h] . K) V over the keys max(0, start[s]) .. position of r
+ *   (causal = 1) or .. kv_len[s] - 1 (causal = 0); start NULL: 0.  Query head h reads key/value head
+ *   h / (n_q_heads / n_kv_heads).  fp32 scores, softmax statistics and sums; probabilities enter the second product
+ *   in the cache's type.  lse (optional, fp32 by l_ts, l_hs): natural log of the sum of exponentials.  A row that
+ *   sees no key: zeros, lse = -inf.  What a row does not see (values of NaN or infinity included) does not change
+ *   it.  head_dim 64, 128 or 256; caches 16-byte aligned with strides that are multiples of 8; scale > 0, finite.
+ *   ws (16-byte aligned, >= ospo_paged_attn_ws_bytes, contents don't matter): partial results of rows whose keys
+ *   were split; calls that may run at once need one each.  Deterministic. */
+int ospo_rotary(const void* q, long q_ts, long q_hs, void* q_out, long qo_ts, long qo_hs, int n_q_heads, const void* k,
+                long k_ts, long k_hs, void* k_out, long ko_ts, long ko_hs, int n_k_heads, int n, int head_dim,
+                int rot_dim, int interleaved, const int* positions, const float* cos_tab, const float* sin_tab,
+                int n_pos, int backward, int dtype, hipStream_t stream);
+int ospo_paged_append(const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs, const void* q,
+                      long q_ts, long q_hs, void* q_out, long qo_ts, long qo_hs, int n, int n_q_heads, int n_kv_heads,
+                      int head_dim, void* k_cache, void* v_cache, long page_stride, long head_stride, long slot_stride,
+                      int n_pages, int page_size, const int* block_table, int max_pages, const int* q_start,
+                      const int* kv_len, int n_seqs, const float* cos_tab, const float* sin_tab, int n_pos,
+                      int rot_dim, int interleaved, int dtype, hipStream_t stream);
+size_t ospo_paged_attn_ws_bytes(int n, int n_seqs, int n_q_heads, int n_kv_heads, int head_dim, int page_size,
+                                int max_pages);
+int ospo_paged_attn(const void* q, long q_ts, long q_hs, const void* k_cache, const void* v_cache, long page_stride,
+                    long head_stride, long slot_stride, int n_pages, int page_size, const int* block_table,
+                    int max_pages, const int* q_start, const int* kv_len, const int* start, int n_seqs, int n,
+                    int n_q_heads, int n_kv_heads, int head_dim, float scale, int causal, void* out, long o_ts,
+                    long o_hs, float* lse, long l_ts, long l_hs, int dtype, void* ws, size_t ws_bytes,
+                    hipStream_t stream);
+
 /* ------------------------------------------------------- VQ image tokenizer ---
  * janus/models/vq_model.py Encoder (:46-124) + quant_conv + VectorQuantizer
  * (:236-282) = gen_vision_model.encode, called per image at ospo/wrapper/train.py:246-264.  fp32

@@ -92,6 +92,12 @@ SIGNATURES = {
     "ospo_cfg_sample": [P, I, I, I, F, F, P, P, I, P, P, P, P],
     "ospo_embed_rows": [P, L, P, I, I, P, P],
     "ospo_decode_advance": [P, P, P],
+    "ospo_rotary": [P, L, L, P, L, L, I, P, L, L, P, L, L, I, I, I, I, I, P, P, P, I, I, I, P],
+    "ospo_paged_append": [P, L, L, P, L, L, P, L, L, P, L, L, I, I, I, I, P, P, L, L, L, I, I, P, I, P, P, I, P, P,
+                          I, I, I, I, P],
+    "ospo_paged_attn_ws_bytes": [I, I, I, I, I, I, I],
+    "ospo_paged_attn": [P, L, L, P, P, L, L, L, I, I, P, I, P, P, P, I, I, I, I, I, F, I, P, L, L, P, L, L, I, P, Z,
+                        P],
     "ospo_vq_conv2d": [P, I, I, I, I, P, I, I, I, I, I, I, I, I, P, P, P, P],
     "ospo_vq_bmm_nt": [P, P, I, I, I, I, P, P],
     "ospo_vq_groupnorm_ws_bytes": [I, I],
@@ -112,7 +118,7 @@ ABLATION_SIGNATURES = {"ospo_set_gemm_variant": [I], "ospo_set_gemv_variant": [I
                        "ospo_set_skinny_variant": [I], "ospo_gemm_set_debug_buffer": [P],
                        "ospo_attn_set_stamps": [P]}
 
-RESTYPES = {"ospo_ws_counter_bytes": c_size_t, "ospo_gemm_nt_ws_bytes": c_size_t, "ospo_row_dot_sum_ws_bytes": c_size_t, "ospo_lora_gdb_ws_bytes": c_size_t, "ospo_flash_attn_bwd_ws_bytes": c_size_t, "ospo_lora_skinny_ws_bytes": c_size_t, "ospo_mx8_scale_bytes": c_size_t, "ospo_decode_gemv_ws_bytes": c_size_t, "ospo_decode_linear_ws_bytes": c_size_t, "ospo_vq_groupnorm_ws_bytes": c_size_t, "ospo_dropout_hash": c_uint}
+RESTYPES = {"ospo_ws_counter_bytes": c_size_t, "ospo_gemm_nt_ws_bytes": c_size_t, "ospo_row_dot_sum_ws_bytes": c_size_t, "ospo_lora_gdb_ws_bytes": c_size_t, "ospo_flash_attn_bwd_ws_bytes": c_size_t, "ospo_lora_skinny_ws_bytes": c_size_t, "ospo_mx8_scale_bytes": c_size_t, "ospo_decode_gemv_ws_bytes": c_size_t, "ospo_decode_linear_ws_bytes": c_size_t, "ospo_vq_groupnorm_ws_bytes": c_size_t, "ospo_paged_attn_ws_bytes": c_size_t, "ospo_dropout_hash": c_uint}
 
 _lib = None
 

@@ -1,0 +1,663 @@
+// Attention of new tokens over a paged key/value cache.
+//
+//   o[r] = sum_j p_rj v_j / sum_j p_rj,  p_rj = exp(scale q_r . k_j),  start <= j <= position of r
+//
+// One pass over the keys with the running maximum and sum of the softmax.  The query heads that share a
+// key/value head are rows of one tile (row = token * group + head in group), so a key is read once for all of
+// them.  S^T = K Q^T puts a query on a lane: its scores are the lane's registers, and those registers are the
+// operand of O^T += V^T P^T.
+//
+// Work is cut into items (sequence, row tile, key/value head, key chunk).  The grid is sized from shapes alone;
+// a workgroup finds its item from the lengths on the device, which also choose the chunk size, so that a captured
+// call follows the lengths at its replay.  An item whose keys are one chunk writes its rows; others write
+// (maximum, sum, O) in fp32 and a second launch joins them in chunk order: no atomics, the same bits each time.
+#include <math.h>
+
+#include "paged.h"
+
+namespace {
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+constexpr float NONE = -1e30f;  // running maximum before any key: finite, so that exp2(m - m) is 1
+
+struct PagedArgs {
+  const void* q;
+  const void* kc;
+  const void* vc;
+  void* o;
+  float* lse;
+  const int* bt;
+  const int* qs;
+  const int* kl;
+  const int* st;
+  long q_ts, q_hs, o_ts, o_hs, l_ts, l_hs;
+  long c_ps, c_hs, c_ts;
+  int rows, S, Hk, n_pages, max_pages, most;
+  FDiv g, ps;      // query heads per key/value head, page size
+  float cs;        // scale * log2 e
+  int causal;
+  int qvec, ovec;  // q rows and o rows allow 16-byte access
+  int slots;       // workgroups that run at once: what a split aims for
+  int split;       // 0: every item is one chunk
+  long items;      // of the launch (an upper bound of those there are)
+  float* ws;       // partial O [item][BM][D], then (m, l) [item][BM][2]
+  long ws_ml;      // offset of the latter, floats
+};
+
+// ---------------------------------------------------------------- items
+// units: key blocks of KU that the sequence's longest row sees (every tile of it is cut at the same places)
+__device__ __forceinline__ void seq_tiles(const Seq& q, const FDiv& g, int BM, int KU, int& tiles, int& units) {
+  const long r = (long)q.n * (int)g.d;
+  tiles = (int)((r + BM - 1) / BM);
+  units = q.kv > q.st ? (q.kv + KU - 1) / KU - q.st / KU : 0;
+  if (units < 1) units = 1;
+}
+__device__ __forceinline__ long wave_sum_l(long v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+__device__ __forceinline__ int wave_max_i(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
+  return v;
+}
+// Key blocks of a chunk.  With L = all work / slots: where the tiles alone fill the slots, chunks of at most L / 4
+// even out the last round (only the long sequences are cut once there are many tiles); where they do not, the
+// smallest chunk that keeps one round.
+__device__ int pick_chunk(const PagedArgs& a, int lane, int BM, int KU) {
+  long total = 0, base = 0;
+  int most = 1;
+  for (int s0 = 0; s0 < a.S; s0 += 64) {
+    const int s = s0 + lane;
+    if (s < a.S) {
+      const Seq q = load_seq(a.qs, a.kl, a.st, s, a.rows, a.most);
+      int t, u;
+      seq_tiles(q, a.g, BM, KU, t, u);
+      if (t) most = max(most, u);
+      total += (long)t * u;
+      base += t;
+    }
+  }
+  total = wave_sum_l(total) * a.Hk;
+  base = wave_sum_l(base) * a.Hk;
+  most = wave_max_i(most);
+  if (!a.split) return most;
+  const long L = (total + a.slots - 1) / a.slots;
+  if (base > a.slots) {
+    const long c = base >= 4l * a.slots ? L : (L + 3) / 4;
+    return (int)min((long)most, max(1l, c));
+  }
+  int C = (int)min((long)most, max(1l, L));
+  while (C < most) {
+    long n = 0;
+    for (int s0 = 0; s0 < a.S; s0 += 64) {
+      const int s = s0 + lane;
+      if (s < a.S) {
+        const Seq q = load_seq(a.qs, a.kl, a.st, s, a.rows, a.most);
+        int t, u;
+        seq_tiles(q, a.g, BM, KU, t, u);
+        n += (long)t * ((u + C - 1) / C);
+      }
+    }
+    if (wave_sum_l(n) * a.Hk <= a.slots) break;
+    C += (C + 7) / 8;
+  }
+  return min(C, most);
+}
+
+struct Item {
+  Seq q;
+  int seq, tile, head, chunk, nch, cs, u0, units;
+  long first;  // item index of chunk 0 of this (tile, head); chunks are `step` apart
+  int step;
+};
+// Order of a sequence's items: heads fastest over the XCDs (hb = largest power of two <= 8 that divides Hk, so a
+// key/value head stays on its XCDs' L2), then chunks, then tiles from the last (the longest rows first), then the
+// remaining heads.
+// mode 0: find the item; mode 1: find (tile, head) pair number `id` (the joining launch)
+__device__ bool find_item(const PagedArgs& a, long id, int lane, int BM, int KU, int mode, Item& it) {
+  const int C = pick_chunk(a, lane, BM, KU);
+  long before = 0, ibefore = 0;
+  for (int s0 = 0; s0 < a.S; s0 += 64) {
+    const int s = s0 + lane;
+    Seq q{0, 0, 0, 0};
+    int t = 0, u = 1, nch = 1;
+    if (s < a.S) {
+      q = load_seq(a.qs, a.kl, a.st, s, a.rows, a.most);
+      seq_tiles(q, a.g, BM, KU, t, u);
+      nch = (u + C - 1) / C;
+    }
+    const long mine = (long)t * a.Hk * (mode ? 1 : nch);
+    long inc = mine, iinc = (long)t * a.Hk * nch;
+    const long imine = iinc;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const long x = __shfl_up(inc, o, 64), y = __shfl_up(iinc, o, 64);
+      if (lane >= o) inc += x, iinc += y;
+    }
+    const bool here = id >= before + inc - mine && id < before + inc;
+    const unsigned long long b = __ballot(here);
+    if (b) {
+      const int w = __ffsll(b) - 1;
+      it.q.q0 = __shfl(q.q0, w, 64), it.q.n = __shfl(q.n, w, 64);
+      it.q.kv = __shfl(q.kv, w, 64), it.q.st = __shfl(q.st, w, 64);
+      it.seq = s0 + w;
+      const int tiles = __shfl(t, w, 64);
+      it.units = __shfl(u, w, 64), it.nch = __shfl(nch, w, 64);
+      const long at = id - before - __shfl(inc - mine, w, 64);
+      const long ibase = ibefore + __shfl(iinc - imine, w, 64);
+      int hb = 8;
+      while (a.Hk % hb) hb >>= 1;
+      const int per = mode ? tiles : tiles * it.nch;
+      const int hl = (int)(at % hb);
+      const long z = at / hb;
+      const int hh = (int)(z / per), x = (int)(z % per);
+      it.head = hh * hb + hl;
+      it.tile = tiles - 1 - (mode ? x : x / it.nch);
+      it.chunk = mode ? 0 : x % it.nch;
+      it.cs = (it.units + it.nch - 1) / it.nch;
+      it.u0 = it.q.st / KU;
+      it.first = ibase + ((long)hh * tiles * it.nch + (long)(tiles - 1 - it.tile) * it.nch) * hb + hl;
+      it.step = hb;
+      return true;
+    }
+    before += __shfl(inc, 63, 64);
+    ibefore += __shfl(iinc, 63, 64);
+  }
+  return false;
+}
+// one past the last key that any row of the tile sees
+__device__ __forceinline__ int tile_end(const PagedArgs& a, const Item& it, int BM) {
+  if (!a.causal) return it.q.kv;
+  const int last = min((it.tile + 1) * BM, it.q.n * (int)a.g.d) - 1;
+  return max(0, it.q.kv - it.q.n + fdiv(last, a.g) + 1);
+}
+
+// ---------------------------------------------------------------- types
+template <typename T>
+struct Frag;
+template <>
+struct Frag<bf16> {
+  typedef bf16x8 v8;
+  static constexpr unsigned EXP = 0x7f80, MAN = 0x007f;
+  __device__ static f32x16 mma(const v8& x, const v8& y, const f32x16& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0);
+  }
+};
+template <>
+struct Frag<f16> {
+  typedef f16x8 v8;
+  static constexpr unsigned EXP = 0x7c00, MAN = 0x03ff;
+  __device__ static f32x16 mma(const v8& x, const v8& y, const f32x16& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0);
+  }
+};
+
+// LDS images are [key][D] with the 16-byte chunks of a row swizzled so that both the row reads of K (32 rows, one
+// chunk) and the transposed reads of V (4 rows x 4 chunks) meet every bank once: 256-byte rows rotate by
+// 4 (r & 3) + ((r >> 2) & 3) over 16 chunks, 128-byte rows (two share the banks) by 4 ((r >> 1) & 1) + ((r >> 2) & 3)
+// over 8.
+template <int D>
+__device__ __forceinline__ int swz(int r) {
+  return D >= 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+}
+
+// 16 bytes a lane from global memory to LDS (wave-uniform destination + 16 lane), without registers
+__device__ __forceinline__ void dma16(const void* src, char* dst) {
+  __builtin_amdgcn_global_load_lds(src, (LDS_AS void*)dst, 16, 0, 0);
+}
+// transposed read: a group of 16 lanes reads 4 rows x 16 columns, lane i gets column i
+__device__ __forceinline__ i16x4 read_tr(const char* src) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS i16x4*)src);
+}
+
+__device__ __forceinline__ float other_half(float x) {  // the value of lane ^ 32
+  const unsigned u = __float_as_uint(x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+// N finished values of a row from column d0 on: divided by the sum (a row that saw no key: zeros), rounded once
+template <typename T, int N>
+__device__ __forceinline__ void store_row(const PagedArgs& a, int tok, int hd, int d0, const float* x, float M, float L) {
+  const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;
+  T* p = (T*)a.o + (long)tok * a.o_ts + (long)hd * a.o_hs + d0;
+  struct alignas(2 * N) { T v[N]; } y;
+#pragma unroll
+  for (int i = 0; i < N; ++i) y.v[i] = (T)(L == 0.f ? 0.f : x[i] * inv);
+  if (a.ovec) {
+    *reinterpret_cast<decltype(y)*>(p) = y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = y.v[i];
+  }
+  if (a.lse && d0 == 0)
+    a.lse[(long)tok * a.l_ts + (long)hd * a.l_hs] = L == 0.f ? -INFINITY : (M + __log2f(L)) * LN2;
+}
+
+constexpr int pitch_of(int D) { return D + 4; }  // floats of a staged output row
+
+template <int D, int WR, int WK, int KT>
+constexpr int lds_bytes() {
+  const int kv = WK * 2 * KT * D * 2;
+  const int out = WR * WK * 32 * pitch_of(D) * 4 + WR * WK * 32 * 8;
+  return kv > out ? kv : out;
+}
+
+// WR waves along the rows (32 RB each), WK along the keys; a wave's key tiles are KT keys wide.
+template <typename T, int D, int RB, int WR, int WK, int KT>
+__global__ __launch_bounds__(64 * WR * WK) void paged_attn_kernel(const PagedArgs a) {
+  using F = Frag<T>;
+  using v8 = typename F::v8;
+  constexpr int BM = 32 * RB * WR, KU = KT * WK, NT = 64 * WR * WK;
+  constexpr int ROWB = D * 2, CH = D / 8;
+  constexpr int KS = D / 16;  // d steps of S
+  constexpr int DC = D / 32;  // d chains of O
+  constexpr int KB = KT / 32;  // key blocks of S
+  __shared__ __attribute__((aligned(16))) char smem[lds_bytes<D, WR, WK, KT>()];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wr = wave % WR, wk = wave / WR;
+  const int hi = lane >> 5, l32 = lane & 31;
+
+  Item it;
+  if (!find_item(a, blockIdx.x, lane, BM, KU, 0, it)) return;
+  const int R = it.q.n * (int)a.g.d;  // rows of the sequence
+  const int ub = it.u0 + it.chunk * it.cs;
+  const int kb = ub * KU;  // the chunk's keys: kb (a multiple of KU) .. ke - 1
+  const int ke = min(min(ub + it.cs, it.u0 + it.units) * KU, tile_end(a, it, BM));
+  const bool part = it.nch > 1;
+  if (part && it.chunk > 0 && kb >= ke) return;  // the joining launch counts the same chunks
+  const int row0 = it.tile * BM + wr * 32 * RB;
+
+  // rows of this lane: row0 + 32 b + l32 (rows behind the last repeat it and are not stored)
+  v8 qf[RB][KS];
+  int lim[RB], low = 0x7fffffff, high = -1;
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    const int r = min(row0 + 32 * b + l32, R - 1);
+    const int tok = fdiv(r, a.g), hd = it.head * (int)a.g.d + r - tok * (int)a.g.d;
+    lim[b] = a.causal ? it.q.kv - it.q.n + tok : it.q.kv - 1;
+    low = min(low, lim[b]);
+    high = max(high, lim[b]);
+    const T* p = (const T*)a.q + (long)(it.q.q0 + tok) * a.q_ts + (long)hd * a.q_hs + 8 * hi;
+    if (a.qvec) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) qf[b][ks] = *reinterpret_cast<const v8*>(p + 16 * ks);
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) qf[b][ks][i] = p[16 * ks + i];
+    }
+  }
+  // the wave's smallest and largest limit: tiles behind the latter are left out, tiles up to the former whole
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) {
+    low = min(low, __shfl_xor(low, s, 64));
+    high = max(high, __shfl_xor(high, s, 64));
+  }
+  low = __builtin_amdgcn_readfirstlane(low);
+  high = __builtin_amdgcn_readfirstlane(row0 < R ? high : -1);
+
+  f32x16 o[RB][DC];
+  float m[RB], l[RB];
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    m[b] = NONE, l[b] = 0.f;
+#pragma unroll
+    for (int c = 0; c < DC; ++c)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[b][c][r] = 0.f;
+  }
+
+  char* kl = smem + wk * 2 * KT * ROWB;  // this key group's K image, then V's
+  char* vl = kl + KT * ROWB;
+  const T* kc = (const T*)a.kc + (long)it.head * a.c_hs;
+  const T* vc = (const T*)a.vc + (long)it.head * a.c_hs;
+  const int* bt = a.bt + (long)it.seq * a.max_pages;
+  const int steps = ke > kb ? (ke - kb + KU - 1) / KU : 0;
+  for (int t = 0; t < steps; ++t) {
+    const int k0 = kb + t * KU + wk * KT;  // this wave's tile
+    __syncthreads();
+    if (k0 < ke) {
+      constexpr int RPP = 1024 / ROWB;  // rows of a 1-KiB piece (one LDS-DMA of the wave)
+#pragma unroll
+      for (int p = 0; p < KT / RPP / WR; ++p) {
+        const int piece = wr + WR * p;
+        const int row = piece * RPP + lane / CH;
+        const int key = min(k0 + row, ke - 1);
+        const int pi = fdiv(key, a.ps);
+        const int page = min(max(bt[pi], 0), a.n_pages - 1);
+        const long off = (long)page * a.c_ps + (long)(key - pi * (int)a.ps.d) * a.c_ts +
+                         (((lane % CH) ^ swz<D>(row)) << 3);
+        dma16(kc + off, kl + piece * 1024);
+        dma16(vc + off, vl + piece * 1024);
+      }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (k0 >= ke || k0 > high) continue;
+    const bool mask = k0 < it.q.st || k0 + KT - 1 > low;
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      f32x16 s[KB];
+#pragma unroll
+      for (int kk = 0; kk < KB; ++kk) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[kk][r] = 0.f;
+        const int row = 32 * kk + l32;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const v8 kf = *reinterpret_cast<const v8*>(kl + row * ROWB + (((2 * ks + hi) ^ swz<D>(row)) << 4));
+          s[kk] = F::mma(kf, qf[b][ks], s[kk]);
+        }
+      }
+      if (mask) {
+#pragma unroll
+        for (int kk = 0; kk < KB; ++kk)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int key = k0 + 32 * kk + (r & 3) + 8 * (r >> 2) + 4 * hi;
+            s[kk][r] = key > lim[b] || key < it.q.st ? -INFINITY : s[kk][r];
+          }
+      }
+      float mx = s[0][0];
+#pragma unroll
+      for (int kk = 0; kk < KB; ++kk)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kk][r]);
+      mx = fmaxf(mx, other_half(mx));
+      const float mn = fmaxf(m[b], mx * a.cs);
+      const float alpha = __builtin_amdgcn_exp2f(m[b] - mn);
+      m[b] = mn;
+      float sum = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < KB; ++kk)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[kk][r] = __builtin_amdgcn_exp2f(fmaf(s[kk][r], a.cs, -mn));
+          sum += s[kk][r];
+        }
+      l[b] = l[b] * alpha + sum + other_half(sum);
+      // P in the cache's type (rounded to nearest: the matrix unit's operand; the sum above keeps fp32)
+      v8 pt[KT / 16];
+#pragma unroll
+      for (int u = 0; u < KT / 16; ++u)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pt[u][i] = (T)s[u >> 1][8 * (u & 1) + i];
+      auto vfrag = [&](int c, int u) __attribute__((always_inline)) {
+        const int G = lane >> 4, li = lane & 15;
+        const int r1 = 16 * u + 4 * hi + (li >> 2), r2 = r1 + 8;
+        const int ch = 4 * c + 2 * (G & 1) + ((li & 3) >> 1), h8 = (li & 1) << 3;
+        const i16x4 x = read_tr(vl + r1 * ROWB + ((ch ^ swz<D>(r1)) << 4) + h8);
+        const i16x4 y = read_tr(vl + r2 * ROWB + ((ch ^ swz<D>(r2)) << 4) + h8);
+        return i16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+      };
+      if (!mask) {
+#pragma unroll
+        for (int c = 0; c < DC; ++c) {
+          o[b][c] *= alpha;
+#pragma unroll
+          for (int u = 0; u < KT / 16; ++u) o[b][c] = F::mma(__builtin_bit_cast(v8, vfrag(c, u)), pt[u], o[b][c]);
+        }
+      } else {
+        // A masked key has p = 0, but 0 times an infinity or NaN in its value would reach the row all the same.
+        // The tile's product is formed apart; where it is not finite, it is formed again with those values as
+        // zeros, and what rows that see them get is added: +inf, -inf or NaN, found by a product with the mask.
+#pragma unroll
+        for (int c = 0; c < DC; ++c) {
+          f32x16 x;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) x[r] = 0.f;
+#pragma unroll
+          for (int u = 0; u < KT / 16; ++u) x = F::mma(__builtin_bit_cast(v8, vfrag(c, u)), pt[u], x);
+          float bad = 0.f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) bad = fmaf(x[r], 0.f, bad);
+          if (__ballot(bad != 0.f)) {
+            f32x16 up, dn;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[r] = up[r] = dn[r] = 0.f;
+            for (int u = 0; u < KT / 16; ++u) {
+              const i16x8 v = vfrag(c, u);
+              v8 fin, isup, isdn, seen;
+              const v8 pu = u == 0 ? pt[0] : u == 1 ? pt[1] : KT > 32 && u == 2 ? pt[KT > 32 ? 2 : 0] : pt[KT > 32 ? 3 : 1];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const short e = v[i];  // (a copy: a bit cast of the vector's element itself takes element 0)
+                const unsigned bits = (unsigned short)e;
+                const bool odd = (bits & F::EXP) == F::EXP, nan = odd && (bits & F::MAN);
+                fin[i] = odd ? (T)0.f : __builtin_bit_cast(T, e);
+                isup[i] = nan || (odd && !(bits & 0x8000)) ? (T)1.f : (T)0.f;
+                isdn[i] = nan || (odd && (bits & 0x8000)) ? (T)1.f : (T)0.f;
+                const int key = k0 + 16 * u + 4 * hi + (i & 3) + 8 * (i >> 2);
+                seen[i] = key > lim[b] || key < it.q.st ? (T)0.f : (T)1.f;
+              }
+              x = F::mma(fin, pu, x);
+              up = F::mma(isup, seen, up);
+              dn = F::mma(isdn, seen, dn);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              if (up[r] > 0.f) x[r] += INFINITY;
+              if (dn[r] > 0.f) x[r] -= INFINITY;
+            }
+          }
+          o[b][c] = o[b][c] * alpha + x;
+        }
+      }
+    }
+  }
+
+  // Join the key groups and store: rows through LDS, 16 bytes a lane.
+  const int R0 = it.tile * BM;
+  constexpr int PITCH = pitch_of(D);
+  float* ml = reinterpret_cast<float*>(smem + WR * WK * 32 * PITCH * 4);  // [wave][row] (m, l)
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    __syncthreads();
+    if (hi == 0) ml[(wave * 32 + l32) * 2] = m[b], ml[(wave * 32 + l32) * 2 + 1] = l[b];
+    __syncthreads();
+    float M = m[b];
+#pragma unroll
+    for (int k = 0; k < WK; ++k) M = fmaxf(M, ml[((k * WR + wr) * 32 + l32) * 2]);
+    const float w = __builtin_amdgcn_exp2f(m[b] - M);
+    float* mine = reinterpret_cast<float*>(smem) + (wave * 32 + l32) * PITCH;
+#pragma unroll
+    for (int c = 0; c < DC; ++c)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        f32x4 x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = o[b][c][4 * k + i] * w;
+        *reinterpret_cast<f32x4*>(mine + 32 * c + 8 * k + 4 * hi) = x;
+      }
+    __syncthreads();
+    constexpr int TPR = D / 8;
+    for (int idx = threadIdx.x; idx < WR * 32 * TPR; idx += NT) {
+      const int lr = idx / TPR, d0 = (idx % TPR) * 8;
+      const int w_ = lr / 32, r32 = lr % 32;
+      const int r = R0 + w_ * 32 * RB + 32 * b + r32;
+      if (r >= R) continue;
+      float x[8], M2 = NONE, L = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < WK; ++k) M2 = fmaxf(M2, ml[((k * WR + w_) * 32 + r32) * 2]);
+#pragma unroll
+      for (int k = 0; k < WK; ++k) {
+        const int wv = k * WR + w_;
+        L += ml[(wv * 32 + r32) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(wv * 32 + r32) * 2] - M2);
+        const float* y = reinterpret_cast<const float*>(smem) + (wv * 32 + r32) * PITCH + d0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] += y[i];
+      }
+      const int tok = fdiv(r, a.g), hd = it.head * (int)a.g.d + r - tok * (int)a.g.d;
+      if (part) {
+        const long slot = (long)blockIdx.x * BM + (r - R0);
+        float* y = a.ws + slot * D + d0;
+        *reinterpret_cast<f32x4*>(y) = f32x4{x[0], x[1], x[2], x[3]};
+        *reinterpret_cast<f32x4*>(y + 4) = f32x4{x[4], x[5], x[6], x[7]};
+        if (d0 == 0) *reinterpret_cast<f32x2*>(a.ws + a.ws_ml + slot * 2) = f32x2{M2, L};
+      } else {
+        store_row<T, 8>(a, it.q.q0 + tok, hd, d0, x, M2, L);
+      }
+    }
+  }
+}
+
+// Joins the chunks of a (tile, head): D / 4 threads a row.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a, int BM, int KU) {
+  Item it;
+  const int lane = threadIdx.x & 63;
+  if (!find_item(a, blockIdx.x, lane, BM, KU, 1, it)) return;
+  if (it.nch <= 1) return;
+  constexpr int TPR = D / 4;
+  const int R = it.q.n * (int)a.g.d;
+  const int lr = blockIdx.y * (256 / TPR) + threadIdx.x / TPR, r = it.tile * BM + lr;
+  if (lr >= BM || r >= R) return;
+  const int d0 = (threadIdx.x % TPR) * 4;
+  const int end = min(tile_end(a, it, BM), (it.u0 + it.units) * KU);
+  const int left = end - it.u0 * KU;
+  const int n = left > 0 ? (left + it.cs * KU - 1) / (it.cs * KU) : 1;  // chunks that wrote
+  if (it.first + (long)(n - 1) * it.step >= a.items) return;  // only where q_start descends
+  const float* ml = a.ws + a.ws_ml;
+  float M = NONE;
+  for (int c = 0; c < n; ++c) M = fmaxf(M, ml[((it.first + (long)c * it.step) * BM + lr) * 2]);
+  float x[4] = {0.f, 0.f, 0.f, 0.f}, L = 0.f;
+  for (int c = 0; c < n; ++c) {
+    const long slot = (it.first + (long)c * it.step) * BM + lr;
+    const f32x2 p = *reinterpret_cast<const f32x2*>(ml + slot * 2);
+    const f32x4 y = *reinterpret_cast<const f32x4*>(a.ws + slot * D + d0);
+    const float w = __builtin_amdgcn_exp2f(p[0] - M);
+    L += p[1] * w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] += y[i] * w;
+  }
+  const int tok = fdiv(r, a.g), hd = it.head * (int)a.g.d + r - tok * (int)a.g.d;
+  store_row<T, 4>(a, it.q.q0 + tok, hd, d0, x, M, L);
+}
+
+// ---------------------------------------------------------------- host
+struct Plan {
+  int BM, KU;
+  long pairs, items;  // upper bounds: (tile, head) pairs and items
+  int slots, split;
+  size_t ml_off, bytes;
+};
+
+int device_cus() {
+  static int cus[64];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  if (!cus[dev]) {
+    int n = 0;
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 1) n = 256;
+    cus[dev] = n;
+  }
+  return cus[dev];
+}
+
+// Few rows for each sequence and key/value head: 32-row tiles whose four waves share out the keys.  Otherwise
+// 128-row tiles whose four waves share the keys.
+bool few_rows(long rows, int S, int g) { return rows * g <= 32l * S; }
+
+Plan make_plan(long rows, int S, int Hq, int Hk, int D, long most) {
+  Plan p;
+  const int g = Hq / Hk;
+  const bool few = few_rows(rows, S, g);
+  p.BM = few ? 32 : 128;
+  p.KU = few ? (D > 128 ? 128 : 128) : 64;
+  p.pairs = (rows * g / p.BM + S) * Hk;
+  p.slots = device_cus() * 2;
+  const long least = (rows * g + p.BM - 1) / p.BM * Hk;
+  p.split = most > p.KU && least < 8l * p.slots;
+  p.items = p.split ? p.pairs + 4l * p.slots : p.pairs;
+  p.ml_off = p.split ? (size_t)p.items * p.BM * D : 0;
+  p.bytes = p.split ? (p.ml_off + (size_t)p.items * p.BM * 2) * 4 : 0;
+  return p;
+}
+
+template <typename T, int D>
+int launch(PagedArgs& a, const Plan& p, hipStream_t st) {
+  const dim3 grid((unsigned)p.items);
+  if (p.BM == 32)
+    paged_attn_kernel<T, D, 1, 1, 4, 32><<<grid, 256, 0, st>>>(a);
+  else
+    paged_attn_kernel<T, D, 1, 4, 1, 64><<<grid, 256, 0, st>>>(a);
+  OSPO_CHECK_LAUNCH();
+  if (p.split) {
+    constexpr int RPB = 256 / (D / 4);
+    paged_join_kernel<T, D><<<dim3((unsigned)p.pairs, (unsigned)((p.BM + RPB - 1) / RPB)), 256, 0, st>>>(a, p.BM, p.KU);
+    OSPO_CHECK_LAUNCH();
+  }
+  return OSPO_OK;
+}
+
+bool shapes_ok(int n, int S, int Hq, int Hk, int D, int n_pages, int page_size, int max_pages) {
+  return n >= 0 && S >= 0 && Hk >= 1 && Hq >= Hk && Hq % Hk == 0 && Hq <= 4096 && n_pages >= 0 && page_size >= 1 &&
+         max_pages >= 0 && (long)max_pages * page_size <= 0x7fff0000L && (long)n * (Hq / Hk) <= 0x7fffff00L;
+}
+
+}  // namespace
+
+extern "C" size_t ospo_paged_attn_ws_bytes(int n, int n_seqs, int n_q_heads, int n_kv_heads, int head_dim,
+                                           int page_size, int max_pages) {
+  if (!shapes_ok(n, n_seqs, n_q_heads, n_kv_heads, head_dim, 0, page_size, max_pages) || !n || !n_seqs) return 0;
+  return make_plan(n, n_seqs, n_q_heads, n_kv_heads, head_dim, (long)page_size * max_pages).bytes;
+}
+
+extern "C" int ospo_paged_attn(const void* q, long q_ts, long q_hs, const void* k_cache, const void* v_cache,
+                               long page_stride, long head_stride, long slot_stride, int n_pages, int page_size,
+                               const int* block_table, int max_pages, const int* q_start, const int* kv_len,
+                               const int* start, int n_seqs, int n, int n_q_heads, int n_kv_heads, int head_dim,
+                               float scale, int causal, void* out, long o_ts, long o_hs, float* lse, long l_ts,
+                               long l_hs, int dtype, void* ws, size_t ws_bytes, hipStream_t stream) {
+  if (!shapes_ok(n, n_seqs, n_q_heads, n_kv_heads, head_dim, n_pages, page_size, max_pages)) return OSPO_ERR_SHAPE;
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return OSPO_ERR_UNSUPPORTED;
+  if (dtype != DT_BF16 && dtype != DT_F16) return OSPO_ERR_UNSUPPORTED;
+  if (!(scale > 0.f) || !(scale < INFINITY) || (causal != 0 && causal != 1)) return OSPO_ERR_ARG;
+  if (n == 0 || n_seqs == 0) return OSPO_OK;
+  if (!q || !out || !q_start || !kv_len) return OSPO_ERR_ARG;
+  const bool keys = max_pages > 0 && n_pages > 0;  // a cache without pages: every row sees nothing
+  if (keys && (!k_cache || !v_cache || !block_table)) return OSPO_ERR_ARG;
+  if (keys && (!aligned16(k_cache) || !aligned16(v_cache))) return OSPO_ERR_ALIGN;
+  if (page_stride % 8 || head_stride % 8 || slot_stride % 8) return OSPO_ERR_ALIGN;
+  const Plan p = make_plan(n, n_seqs, n_q_heads, n_kv_heads, head_dim, (long)page_size * max_pages);
+  if (p.items > 0x7fffffffL || p.pairs > 0x7fffffffL) return OSPO_ERR_SHAPE;
+  if (p.split && (!ws || ws_bytes < p.bytes)) return OSPO_ERR_ARG;
+  if (p.split && !aligned16(ws)) return OSPO_ERR_ALIGN;
+  PagedArgs a{};
+  a.q = q, a.kc = k_cache, a.vc = v_cache, a.o = out, a.lse = lse;
+  a.bt = block_table, a.qs = q_start, a.kl = kv_len, a.st = start;
+  a.q_ts = q_ts, a.q_hs = q_hs, a.o_ts = o_ts, a.o_hs = o_hs, a.l_ts = l_ts, a.l_hs = l_hs;
+  a.c_ps = page_stride, a.c_hs = head_stride, a.c_ts = slot_stride;
+  a.rows = n, a.S = n_seqs, a.Hk = n_kv_heads, a.n_pages = n_pages, a.max_pages = max_pages;
+  a.most = keys ? max_pages * page_size : 0;
+  a.g = make_fdiv((uint32_t)(n_q_heads / n_kv_heads));
+  a.ps = make_fdiv((uint32_t)page_size);
+  a.cs = scale * LOG2E;
+  a.causal = causal;
+  a.qvec = aligned16(q) && q_ts % 8 == 0 && q_hs % 8 == 0;
+  a.ovec = aligned16(out) && o_ts % 8 == 0 && o_hs % 8 == 0;
+  a.slots = p.slots, a.split = p.split, a.items = p.items;
+  a.ws = (float*)ws, a.ws_ml = (long)p.ml_off;
+  if (dtype == DT_BF16) {
+    switch (head_dim) {
+      case 64: return launch<bf16, 64>(a, p, stream);
+      case 128: return launch<bf16, 128>(a, p, stream);
+      default: return launch<bf16, 256>(a, p, stream);
+    }
+  }
+  switch (head_dim) {
+    case 64: return launch<f16, 64>(a, p, stream);
+    case 128: return launch<f16, 128>(a, p, stream);
+    default: return launch<f16, 256>(a, p, stream);
+  }
+}

@@ -5,6 +5,9 @@ in ``_lib``; there is no eager-PyTorch fallback on this path.
 """
 from __future__ import annotations
 
+import contextlib
+import functools
+import math
 from typing import Optional
 
 import torch
@@ -911,3 +914,248 @@ def embed_rows(ids, table, out):
 
 def decode_advance(pos_dev, step_dev):
     call("ospo_decode_advance", _p(pos_dev), _p(step_dev), _s())
+
+
+# ------------------------------------------------------------ paged cache
+_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_ROT_SCALING = ("linear", "ntk", "yarn")
+
+
+def rotary_tables(n_pos: int, rot_dim: int, theta: float, device, scaling: Optional[dict] = None) -> tuple:
+    """(cos, sin) fp32 [n_pos, rot_dim / 2] of the angles p * f_i, f_i = theta^(-2i / rot_dim), formed in 64 bits (at
+    position 10^5 an fp32 angle is off by up to 4e-3 rad).  ``scaling`` stretches them for contexts ``factor`` times
+    as long:
+      {"type": "linear", "factor": s}: f_i / s;
+      {"type": "ntk", "factor": s}: theta * s^(rot_dim / (rot_dim - 2)), so that the slowest pair turns s times slower;
+      {"type": "yarn", "factor": s, "original": L, "beta_fast": 32, "beta_slow": 1, "magnitude": 0.1 ln s + 1}: pairs
+        that turn beta_fast times or more within L keep f_i, those below beta_slow get f_i / s, a linear ramp in
+        between (YaRN, Peng et al. 2023); both tables times the magnitude."""
+    if n_pos < 1 or rot_dim < 2 or rot_dim % 2 or not theta > 0:
+        raise ValueError(f"rotary_tables: n_pos {n_pos}, rot_dim {rot_dim}, theta {theta}")
+    kind, s, mag = None, 1.0, 1.0
+    if scaling is not None:
+        kind, s = scaling.get("type"), float(scaling.get("factor", 1.0))
+        if kind not in _ROT_SCALING or not s >= 1.0 or not math.isfinite(s):
+            raise ValueError(f"rotary_tables: scaling {scaling}: a type of {_ROT_SCALING} and a factor >= 1")
+    if kind == "ntk":
+        if rot_dim < 4:
+            raise ValueError("rotary_tables: ntk scaling needs rot_dim >= 4")
+        theta = theta * s ** (rot_dim / (rot_dim - 2))
+    f = float(theta) ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64, device=device) / rot_dim)
+    if kind == "linear":
+        f = f / s
+    elif kind == "yarn":
+        first, fast, slow = scaling.get("original"), scaling.get("beta_fast", 32.0), scaling.get("beta_slow", 1.0)
+        if not first or first < 1 or not fast > slow > 0:
+            raise ValueError(f"rotary_tables: scaling {scaling}: yarn needs 'original' >= 1 and beta_fast > beta_slow")
+        keep = ((first * f / (2 * math.pi) - slow) / (fast - slow)).clamp(0.0, 1.0)
+        f = f / s * (1 - keep) + f * keep
+        mag = scaling.get("magnitude")
+        mag = 0.1 * math.log(s) + 1.0 if mag is None else float(mag)
+    a = torch.arange(n_pos, dtype=torch.float64, device=device)[:, None] * f
+    return (a.cos() * mag).float(), (a.sin() * mag).float()
+
+
+def _rows3(t: torch.Tensor, name: str, dtype, n: int, d: int) -> tuple:
+    """Strides (token, head) of a [n, heads, d] tensor."""
+    sh, st = t.shape, t.stride()
+    if len(sh) != 3 or sh[0] != n or sh[2] != d or (st[2] != 1 and d > 1):
+        raise ValueError(f"{name}: expected [{n}, heads, {d}] with a contiguous last dimension, got {tuple(sh)} "
+                         f"strides {st}")
+    if t.dtype != dtype:
+        raise ValueError(f"{name}: expected {dtype}, got {t.dtype}")
+    return st[0], st[1]
+
+
+def _ints(t: torch.Tensor, name: str, *shape) -> None:
+    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous int32 tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
+
+
+def _rot_tables(tables, who: str) -> tuple:
+    cos, sin = tables
+    if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or cos.shape != sin.shape
+            or not cos.is_contiguous() or not sin.is_contiguous() or cos.numel() == 0):
+        raise ValueError(f"{who}: tables are two contiguous fp32 [positions, rot_dim / 2] tensors")
+    return cos, sin
+
+
+def _one_device(who: str, *tensors) -> torch.device:
+    """The device of all tensors; refuses host tensors and a mix."""
+    dev = tensors[0].device
+    for t in tensors:
+        if not t.is_cuda:
+            raise ValueError(f"{who}: expected device tensors")
+        if t.device != dev:
+            raise ValueError(f"{who}: tensors on {dev} and {t.device}")
+    return dev
+
+
+def _on(dev: torch.device):
+    """The context that makes ``dev`` current (nothing where it is)."""
+    if dev.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, tables: tuple, *,
+           interleaved: bool = False, backward: bool = False, out: Optional[tuple] = None) -> tuple:
+    """Rotary positions on q [n, q_heads, head_dim] and k [n, kv_heads, head_dim] (or None) of any strides: the first
+    rot_dim = 2 * tables[0].shape[1] elements of a head turn by the tables' row of the token's position (int32 [n],
+    clamped to the tables), in pairs (i, i + rot_dim / 2), or (2i, 2i + 1) with ``interleaved``; the rest is copied.
+    fp32 arithmetic, rounded once to q's type (bf16, fp16, fp32).  ``backward``: q and k are the gradients of the
+    outputs, the result those of the inputs.  ``out`` (q', k'): where to write, the inputs themselves allowed; new
+    tensors by default.  Returns (q', k')."""
+    cos, sin = _rot_tables(tables, "rotary")
+    if q.dim() != 3 or q.dtype not in _CODE:
+        raise ValueError(f"rotary: expected q [n, heads, head_dim] in bf16, fp16 or fp32, got {q.dtype} "
+                         f"{tuple(q.shape)}")
+    n, hq, d = q.shape
+    rot = 2 * cos.shape[1]
+    if hq < 1 or not 1 <= d <= 256 or rot > d:
+        raise ValueError(f"rotary: {hq} heads of {d} (at most 256), of which {rot} turn")
+    qs = _rows3(q, "q", q.dtype, n, d)
+    _ints(positions, "positions", n)
+    hk, ks = 0, (0, 0)
+    if k is not None:
+        ks = _rows3(k, "k", q.dtype, n, d)
+        hk = k.shape[1]
+    if out is None:
+        qo = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
+        ko = None if k is None else torch.empty((n, hk, d), dtype=q.dtype, device=q.device)
+    else:
+        qo, ko = out
+        if qo.shape != q.shape or (ko is None) != (k is None) or (k is not None and ko.shape != k.shape):
+            raise ValueError("rotary: out has other shapes than q and k")
+    qos = _rows3(qo, "out[0]", q.dtype, n, d)
+    kos = (0, 0) if ko is None else _rows3(ko, "out[1]", q.dtype, n, d)
+    dev = _one_device("rotary", q, positions, cos, sin, qo, *(() if k is None else (k, ko)))
+    with _on(dev):
+        call("ospo_rotary", _p(q), qs[0], qs[1], _p(qo), qos[0], qos[1], hq, _p(k), ks[0], ks[1], _p(ko), kos[0],
+             kos[1], hk, n, d, rot, int(interleaved), _p(positions), _p(cos), _p(sin), cos.shape[0], int(backward),
+             _CODE[q.dtype], _s())
+    return qo, ko
+
+
+def _paged(who: str, k_cache, v_cache, block_table, q_start, kv_len, dtype, d: int) -> tuple:
+    """(kv heads, n_pages, page_size, sequences, max_pages, strides) of a paged cache and its tables."""
+    sh, st = k_cache.shape, k_cache.stride()
+    if len(sh) != 4 or sh[3] != d or (st[3] != 1 and d > 1) or k_cache.dtype != dtype:
+        raise ValueError(f"{who}: expected {dtype} caches [pages, kv_heads, page_size, {d}] with a contiguous last "
+                         f"dimension, got {k_cache.dtype} {tuple(sh)}")
+    if v_cache.shape != sh or v_cache.dtype != dtype or v_cache.stride() != st:
+        raise ValueError(f"{who}: k_cache and v_cache differ in shape, type or strides")
+    if sh[1] < 1 or sh[2] < 1:
+        raise ValueError(f"{who}: empty heads or pages in a cache of shape {tuple(sh)}")
+    if block_table.dim() != 2:
+        raise ValueError(f"{who}: block_table is int32 [sequences, pages]")
+    n_seqs, max_pages = block_table.shape
+    _ints(block_table, "block_table", n_seqs, max_pages)
+    _ints(q_start, "q_start", n_seqs + 1)
+    _ints(kv_len, "kv_len", n_seqs)
+    return sh[1], sh[0], sh[2], n_seqs, max_pages, st
+
+
+def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                 block_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, *,
+                 q: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None, rope: Optional[tuple] = None,
+                 interleaved: bool = False) -> Optional[torch.Tensor]:
+    """Store the keys and values [n, kv_heads, head_dim] of a ragged batch in a paged cache
+    [pages, kv_heads, page_size, head_dim] (any page size and strides), keys turned on the way by ``rope`` (tables of
+    ``rotary_tables``; None: stored as they are).  Rows q_start[s] .. q_start[s + 1] - 1 are sequence s's newest
+    tokens, kv_len[s] its length with them, block_table[s] its pages (all int32, read on the device).  With ``q``
+    [n, q_heads, head_dim] its turned copy is returned (``q_out``; may be q itself).  Rows of no sequence are left
+    alone; a row whose position or page does not exist is not stored."""
+    if k.dim() != 3 or k.dtype not in _CODE:
+        raise ValueError(f"paged_append: expected k [n, kv_heads, head_dim] in bf16, fp16 or fp32, got {k.dtype} "
+                         f"{tuple(k.shape)}")
+    n, hk, d = k.shape
+    dt = k.dtype
+    ks, vs = _rows3(k, "k", dt, n, d), _rows3(v, "v", dt, n, d)
+    heads, n_pages, page, n_seqs, max_pages, st = _paged("paged_append", k_cache, v_cache, block_table, q_start, kv_len,
+                                                         dt, d)
+    if v.shape[1] != hk or heads != hk:
+        raise ValueError(f"paged_append: {hk} heads in k, {v.shape[1]} in v, {heads} in the cache")
+    if not 1 <= d <= 256:
+        raise ValueError(f"paged_append: head_dim {d} outside [1, 256]")
+    if rope is None:
+        cos = sin = None
+        rot = n_pos = 0
+    else:
+        cos, sin = _rot_tables(rope, "paged_append")
+        n_pos, rot = cos.shape[0], 2 * cos.shape[1]
+        if rot > d:
+            raise ValueError(f"paged_append: {rot} of {d} elements turn")
+    hq, qs, qos = 0, (0, 0), (0, 0)
+    if q is not None:
+        qs, hq = _rows3(q, "q", dt, n, d), q.shape[1]
+        if q_out is None:
+            q_out = torch.empty((n, hq, d), dtype=dt, device=q.device)
+        elif q_out.shape != q.shape:
+            raise ValueError("paged_append: q_out has another shape than q")
+        qos = _rows3(q_out, "q_out", dt, n, d)
+    elif q_out is not None:
+        raise ValueError("paged_append: q_out without q")
+    dev = _one_device("paged_append", k, v, k_cache, v_cache, block_table, q_start, kv_len,
+                      *(() if q is None else (q, q_out)), *(() if rope is None else (cos, sin)))
+    with _on(dev):
+        call("ospo_paged_append", _p(k), ks[0], ks[1], _p(v), vs[0], vs[1], _p(q), qs[0], qs[1], _p(q_out), qos[0],
+             qos[1], n, hq, hk, d, _p(k_cache), _p(v_cache), st[0], st[1], st[2], n_pages, page, _p(block_table),
+             max_pages, _p(q_start), _p(kv_len), n_seqs, _p(cos), _p(sin), n_pos, rot, int(interleaved), _CODE[dt],
+             _s())
+    return q_out
+
+
+@functools.lru_cache(maxsize=4096)
+def _paged_attn_ws_bytes(index: int, *shape) -> int:
+    """ospo_paged_attn_ws_bytes on the current device ``index``."""
+    return int(query("ospo_paged_attn_ws_bytes", *shape))
+
+
+def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+               q_start: torch.Tensor, kv_len: torch.Tensor, scale: float, *, start: Optional[torch.Tensor] = None,
+               causal: bool = True, out: Optional[torch.Tensor] = None,
+               lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of a ragged batch's new tokens q [n, q_heads, head_dim] (bf16 or fp16; head_dim 64, 128, 256) over a
+    paged cache that holds them already (``paged_append``; same arguments).  Row r of sequence s sees the keys
+    start[s] (default 0) .. its own position, or .. kv_len[s] - 1 with ``causal`` false; query head h reads kv head
+    h // (q_heads // kv_heads).  One call takes chunks and single tokens together.  Returns out [n, q_heads,
+    head_dim]; lse (fp32 [n, q_heads], optional) gets the natural log of each row's sum of exponentials.  A row that
+    sees nothing is zero, its lse -inf; rows of no sequence are left as they were (in a new ``out``: anything)."""
+    if q.dim() != 3 or q.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"paged_attn: expected q [n, heads, head_dim] in bf16 or fp16, got {q.dtype} {tuple(q.shape)}")
+    n, hq, d = q.shape
+    dt = q.dtype
+    if d not in (64, 128, 256):
+        raise ValueError(f"paged_attn: head_dim {d} not in (64, 128, 256)")
+    scale = float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"paged_attn: scale {scale} (positive and finite)")
+    qs = _rows3(q, "q", dt, n, d)
+    hk, n_pages, page, n_seqs, max_pages, st = _paged("paged_attn", k_cache, v_cache, block_table, q_start, kv_len, dt, d)
+    if hq < 1 or hq % hk:
+        raise ValueError(f"paged_attn: {hq} query heads over {hk} key/value heads")
+    if st[0] % 8 or st[1] % 8 or st[2] % 8:
+        raise ValueError(f"paged_attn: cache strides {st} are not multiples of 8")
+    if start is not None:
+        _ints(start, "start", n_seqs)
+    if out is None:
+        out = torch.empty((n, hq, d), dtype=dt, device=q.device)
+    elif out.shape != q.shape:
+        raise ValueError("paged_attn: out has another shape than q")
+    os_ = _rows3(out, "out", dt, n, d)
+    ls = (0, 0)
+    if lse is not None:
+        if lse.dtype != torch.float32 or lse.shape != (n, hq):
+            raise ValueError(f"paged_attn: lse is fp32 [{n}, {hq}], got {lse.dtype} {tuple(lse.shape)}")
+        ls = lse.stride()
+    dev = _one_device("paged_attn", q, k_cache, v_cache, block_table, q_start, kv_len, out,
+                      *(() if start is None else (start,)), *(() if lse is None else (lse,)))
+    with _on(dev):
+        nbytes = _paged_attn_ws_bytes(dev.index, n, n_seqs, hq, hk, d, page, max_pages)
+        # a workspace of its own for each call: freed in stream order, and held by the graph that captures the call
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        call("ospo_paged_attn", _p(q), qs[0], qs[1], _p(k_cache), _p(v_cache), st[0], st[1], st[2], n_pages, page,
+             _p(block_table), max_pages, _p(q_start), _p(kv_len), _p(start), n_seqs, n, hq, hk, d, scale, int(causal),
+             _p(out), os_[0], os_[1], _p(lse), ls[0], ls[1], _CODE[dt], _p(ws), nbytes, _s())
+    return out

@@ -1,0 +1,215 @@
+"""Paged-cache operators without a GPU: the rotary tables, the refusals of the wrappers and of the C entries, and the
+division and the page arithmetic that the kernels use."""
+import math
+
+import pytest
+import torch
+
+from ospo_amd import _lib, ops
+
+BF = torch.bfloat16
+
+
+def test_rotary_tables_plain_and_linear():
+    cos, sin = ops.rotary_tables(50, 16, 10000.0, "cpu")
+    assert cos.dtype == sin.dtype == torch.float32 and cos.shape == sin.shape == (50, 8)
+    for p, i in ((0, 0), (49, 7), (31, 3)):
+        a = p * 10000.0 ** (-2 * i / 16)
+        assert abs(float(cos[p, i]) - math.cos(a)) <= 2.0 ** -24 and abs(float(sin[p, i]) - math.sin(a)) <= 2.0 ** -24
+    half = ops.rotary_tables(50, 16, 10000.0, "cpu", {"type": "linear", "factor": 2.0})
+    assert torch.allclose(half[0][::2], cos[:25], atol=2.0 ** -23) and torch.allclose(half[1][::2], sin[:25], atol=2.0 ** -23)
+
+
+def test_rotary_tables_ntk_and_yarn():
+    s, rot, theta, L = 8.0, 64, 10000.0, 2048
+    f = [theta ** (-2 * i / rot) for i in range(rot // 2)]
+
+    def speed(scaling, mag=1.0):  # angle at position 1 (all are below pi)
+        c, n = ops.rotary_tables(2, rot, theta, "cpu", scaling)
+        assert torch.allclose(c[0], torch.full((rot // 2,), mag)) and bool((n[0] == 0).all())
+        return torch.atan2(n[1].double(), c[1].double())
+
+    ntk = speed({"type": "ntk", "factor": s})
+    assert abs(float(ntk[0]) - 1.0) < 1e-6 and abs(float(ntk[-1]) / (f[-1] / s) - 1) < 1e-4
+    mag = 0.1 * math.log(s) + 1
+    yarn = speed({"type": "yarn", "factor": s, "original": L}, mag)
+    for i in range(rot // 2):
+        turns = L * f[i] / (2 * math.pi)
+        g = min(1.0, max(0.0, (turns - 1) / 31))
+        assert abs(float(yarn[i]) / (f[i] / s * (1 - g) + f[i] * g) - 1) < 1e-4
+    assert torch.allclose(speed({"type": "yarn", "factor": s, "original": L, "magnitude": 1.0}), yarn, atol=1e-6)
+
+
+@pytest.mark.parametrize("kw", [dict(n_pos=0), dict(rot_dim=3), dict(rot_dim=0), dict(theta=0.0),
+                                dict(scaling={"type": "other", "factor": 2.0}),
+                                dict(scaling={"type": "linear", "factor": 0.5}),
+                                dict(scaling={"type": "linear", "factor": math.nan}),
+                                dict(scaling={"type": "ntk", "factor": 2.0}, rot_dim=2),
+                                dict(scaling={"type": "yarn", "factor": 2.0}),
+                                dict(scaling={"type": "yarn", "factor": 2.0, "original": 10, "beta_fast": 1.0})])
+def test_rotary_tables_refusals(kw):
+    a = dict(n_pos=4, rot_dim=8, theta=10000.0, scaling=None)
+    a.update(kw)
+    with pytest.raises(ValueError, match="rotary_tables"):
+        ops.rotary_tables(a["n_pos"], a["rot_dim"], a["theta"], "cpu", a["scaling"])
+
+
+def _rot(**kw):
+    a = dict(q=torch.zeros(3, 4, 64, dtype=BF), k=torch.zeros(3, 2, 64, dtype=BF),
+             positions=torch.zeros(3, dtype=torch.int32), tables=ops.rotary_tables(8, 64, 10000.0, "cpu"), out=None)
+    a.update(kw)
+    return ops.rotary(a["q"], a["k"], a["positions"], a["tables"], out=a["out"])
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(), "device tensors"),
+    (dict(q=torch.zeros(3, 256, dtype=BF)), r"q \[n, heads"),
+    (dict(q=torch.zeros(3, 4, 64, dtype=torch.float64)), "bf16, fp16 or fp32"),
+    (dict(k=torch.zeros(3, 2, 64)), "k: expected"),
+    (dict(k=torch.zeros(2, 2, 64, dtype=BF)), "k: expected"),
+    (dict(q=torch.zeros(3, 64, 4, dtype=BF).transpose(1, 2)), "contiguous last"),
+    (dict(q=torch.zeros(3, 4, 32, dtype=BF), k=None), "of which 64 turn"),
+    (dict(q=torch.zeros(3, 1, 512, dtype=BF), k=None), "at most 256"),
+    (dict(positions=torch.zeros(3, dtype=torch.int64)), "positions"),
+    (dict(positions=torch.zeros(4, dtype=torch.int32)), "positions"),
+    (dict(tables=(torch.zeros(8, 32), torch.zeros(8, 16))), "tables"),
+    (dict(tables=(torch.zeros(8, 32, dtype=BF),) * 2), "tables"),
+    (dict(tables=(torch.zeros(0, 32),) * 2), "tables"),
+    (dict(out=(torch.zeros(3, 4, 64, dtype=BF), None)), "out has other shapes"),
+    (dict(out=(torch.zeros(3, 4, 64), torch.zeros(3, 2, 64, dtype=BF))), r"out\[0\]"),
+])
+def test_rotary_refusals(kw, match):
+    with pytest.raises(ValueError, match=match):
+        _rot(**kw)
+
+
+def _cache(**kw):
+    a = dict(k=torch.zeros(3, 2, 64, dtype=BF), v=torch.zeros(3, 2, 64, dtype=BF), q=torch.zeros(3, 4, 64, dtype=BF),
+             kc=torch.zeros(5, 2, 16, 64, dtype=BF), vc=torch.zeros(5, 2, 16, 64, dtype=BF),
+             table=torch.zeros(2, 3, dtype=torch.int32), q_start=torch.tensor([0, 1, 3], dtype=torch.int32),
+             kv_len=torch.tensor([4, 9], dtype=torch.int32), rope=None, q_out=None, scale=0.1, start=None, out=None,
+             lse=None)
+    a.update(kw)
+    return a
+
+
+SHARED = [
+    (dict(kc=torch.zeros(5, 2, 16, 32, dtype=BF)), "caches"),
+    (dict(kc=torch.zeros(5, 2, 16, 64)), "caches"),
+    (dict(vc=torch.zeros(5, 2, 8, 64, dtype=BF)), "differ"),
+    (dict(vc=torch.zeros(5, 16, 2, 64, dtype=BF).transpose(1, 2)), "differ"),
+    (dict(kc=torch.zeros(5, 2, 0, 64, dtype=BF), vc=torch.zeros(5, 2, 0, 64, dtype=BF)), "empty"),
+    (dict(table=torch.zeros(2, 3, dtype=torch.int64)), "block_table"),
+    (dict(table=torch.zeros(6, dtype=torch.int32)), "block_table"),
+    (dict(q_start=torch.zeros(2, dtype=torch.int32)), "q_start"),
+    (dict(kv_len=torch.zeros(3, dtype=torch.int32)), "kv_len"),
+    (dict(), "device tensors"),
+]
+
+
+@pytest.mark.parametrize("kw,match", SHARED + [
+    (dict(k=torch.zeros(3, 2, 64, dtype=torch.float64)), "bf16, fp16 or fp32"),
+    (dict(v=torch.zeros(3, 1, 64, dtype=BF)), "heads in"),
+    (dict(k=torch.zeros(3, 4, 64, dtype=BF), v=torch.zeros(3, 4, 64, dtype=BF)), "heads in"),
+    (dict(v=torch.zeros(3, 2, 64)), "v: expected"),
+    (dict(rope=(torch.zeros(8, 64),) * 2), "128 of 64"),
+    (dict(q=None, q_out=torch.zeros(3, 4, 64, dtype=BF)), "without q"),
+    (dict(q_out=torch.zeros(3, 2, 64, dtype=BF)), "another shape"),
+])
+def test_paged_append_refusals(kw, match):
+    a = _cache(**kw)
+    with pytest.raises(ValueError, match=match):
+        ops.paged_append(a["k"], a["v"], a["kc"], a["vc"], a["table"], a["q_start"], a["kv_len"], q=a["q"],
+                         q_out=a["q_out"], rope=a["rope"])
+
+
+@pytest.mark.parametrize("kw,match", SHARED + [
+    (dict(q=torch.zeros(3, 4, 64)), "bf16 or fp16"),
+    (dict(q=torch.zeros(3, 4, 96, dtype=BF)), "head_dim 96"),
+    (dict(q=torch.zeros(3, 3, 64, dtype=BF)), "3 query heads over 2"),
+    (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=math.inf), "scale"),
+    (dict(scale=math.nan), "scale"),
+    (dict(start=torch.zeros(3, dtype=torch.int32)), "start"),
+    (dict(out=torch.zeros(3, 4, 32, dtype=BF)), "another shape"),
+    (dict(lse=torch.zeros(3, 4, dtype=BF)), "lse"), (dict(lse=torch.zeros(3, 2)), "lse"),
+    (dict(kc=torch.zeros(5, 2, 16, 68, dtype=BF)[..., :64], vc=torch.zeros(5, 2, 16, 68, dtype=BF)[..., :64]),
+     "multiples of 8"),
+])
+def test_paged_attn_refusals(kw, match):
+    a = _cache(**kw)
+    with pytest.raises(ValueError, match=match):
+        ops.paged_attn(a["q"], a["kc"], a["vc"], a["table"], a["q_start"], a["kv_len"], a["scale"], start=a["start"],
+                       out=a["out"], lse=a["lse"])
+
+
+# ------------------------------------------------------------ the C entries (all return before any launch)
+P16 = 4096  # an aligned address that nothing reads
+
+
+def c_rotary(**kw):
+    a = dict(n=3, d=64, rot=64, il=0, pos=P16, cos=P16, sin=P16, n_pos=8, bwd=0, dt=0, q=P16, qo=P16, hq=2, k=P16,
+             ko=P16, hk=1)
+    a.update(kw)
+    return _lib.lib().ospo_rotary(a["q"], 128, 64, a["qo"], 128, 64, a["hq"], a["k"], 64, 64, a["ko"], 64, 64, a["hk"],
+                                  a["n"], a["d"], a["rot"], a["il"], a["pos"], a["cos"], a["sin"], a["n_pos"], a["bwd"],
+                                  a["dt"], None)
+
+
+@pytest.mark.parametrize("kw,rc", [
+    (dict(n=-1), 1), (dict(rot=63), 1), (dict(rot=66), 1), (dict(rot=0), 1), (dict(d=257, rot=2), 1), (dict(n_pos=0), 1),
+    (dict(hq=0), 1), (dict(hk=-1), 1), (dict(il=2), 5), (dict(bwd=2), 5), (dict(dt=3), 4), (dict(q=None), 5),
+    (dict(k=None), 5), (dict(pos=None), 5), (dict(cos=None), 5), (dict(n=0), 0)])
+def test_c_rotary_refusals(kw, rc):
+    assert c_rotary(**kw) == rc
+
+
+def c_append(**kw):
+    a = dict(k=P16, v=P16, q=P16, qo=P16, n=3, hq=2, hk=1, d=64, kc=P16, vc=P16, pages=4, page=16, bt=P16, maxp=3,
+             qs=P16, kl=P16, S=2, cos=P16, sin=P16, n_pos=8, rot=64, il=0, dt=0)
+    a.update(kw)
+    return _lib.lib().ospo_paged_append(a["k"], 64, 64, a["v"], 64, 64, a["q"], 128, 64, a["qo"], 128, 64, a["n"],
+                                        a["hq"], a["hk"], a["d"], a["kc"], a["vc"], 1024, 1024, 64, a["pages"],
+                                        a["page"], a["bt"], a["maxp"], a["qs"], a["kl"], a["S"], a["cos"], a["sin"],
+                                        a["n_pos"], a["rot"], a["il"], a["dt"], None)
+
+
+@pytest.mark.parametrize("kw,rc", [
+    (dict(n=-1), 1), (dict(hk=0), 1), (dict(page=0), 1), (dict(maxp=-1), 1), (dict(S=-1), 1),
+    (dict(page=2 ** 16, maxp=2 ** 15), 1), (dict(rot=65), 1), (dict(n_pos=0), 1), (dict(il=3), 5), (dict(dt=-1), 4),
+    (dict(k=None), 5), (dict(v=None), 5), (dict(kc=None), 5), (dict(bt=None), 5), (dict(qs=None), 5), (dict(kl=None), 5),
+    (dict(cos=None), 5), (dict(qo=None), 5), (dict(n=0), 0), (dict(S=0), 0)])
+def test_c_append_refusals(kw, rc):
+    assert c_append(**kw) == rc
+
+
+def c_attn(**kw):
+    a = dict(q=P16, kc=P16, vc=P16, ps=1024, hs=1024, ts=64, pages=4, page=16, bt=P16, maxp=3, qs=P16, kl=P16, S=2, n=3,
+             hq=2, hk=1, d=64, scale=0.1, causal=1, out=P16, dt=0, ws=P16, wb=1 << 40)
+    a.update(kw)
+    return _lib.lib().ospo_paged_attn(a["q"], 128, 64, a["kc"], a["vc"], a["ps"], a["hs"], a["ts"], a["pages"], a["page"],
+                                      a["bt"], a["maxp"], a["qs"], a["kl"], None, a["S"], a["n"], a["hq"], a["hk"],
+                                      a["d"], a["scale"], a["causal"], a["out"], 128, 64, None, 0, 0, a["dt"], a["ws"],
+                                      a["wb"], None)
+
+
+@pytest.mark.parametrize("kw,rc", [
+    (dict(n=-1), 1), (dict(hq=3, hk=2), 1), (dict(hk=0), 1), (dict(page=0), 1), (dict(page=2 ** 16, maxp=2 ** 15), 1),
+    (dict(d=96), 4), (dict(dt=2), 4), (dict(scale=0.0), 5), (dict(scale=math.nan), 5), (dict(scale=math.inf), 5),
+    (dict(causal=2), 5), (dict(q=None), 5), (dict(out=None), 5), (dict(kc=None), 5), (dict(bt=None), 5),
+    (dict(qs=None), 5), (dict(kc=P16 + 8), 2), (dict(ts=68), 2), (dict(ps=1025), 2),
+    (dict(maxp=4000, ws=None, wb=0), 5), (dict(maxp=4000, wb=16), 5), (dict(maxp=4000, ws=P16 + 8), 2), (dict(n=0), 0),
+    (dict(S=0), 0)])
+def test_c_attn_refusals(kw, rc):
+    assert c_attn(**kw) == rc
+
+
+def test_division_by_a_multiply_is_exact():
+    """The kernels' n / d (paged.h, make_fdiv and fdiv) for the divisors and dividends where it could go wrong."""
+    for d in list(range(1, 300)) + [511, 512, 513, 1000, 4095, 4096, 65535, 65537, 2 ** 30 - 1, 2 ** 30, 2 ** 31 - 1]:
+        L = max(0, (d - 1).bit_length())
+        m = ((1 << 32) * ((1 << L) - d)) // d + 1
+        assert m < 1 << 32
+        for n in {0, 1, d - 1, d, d + 1, 2 * d - 1, 2 * d, 2 ** 31 - 1, (2 ** 31 - 1) // d * d, (2 ** 31 - 1) // d * d - 1}:
+            if 0 <= n < 2 ** 31:
+                s = ((n * m) >> 32) + n
+                assert s < 1 << 32 and s >> L == n // d, (n, d)
