@@ -163,7 +163,11 @@ def query(name: str, *args) -> int:
 
 
 def call(name: str, *args) -> None:
-    rc = getattr(lib(), name)(*args)
+    check(name, getattr(lib(), name)(*args))
+
+
+def check(name: str, rc: int) -> None:
+    """Raise what status ``rc`` of entry point ``name`` means (0: nothing)."""
     if rc != 0:
         msg = lib().ospo_strerror(rc).decode()
         if rc in (1, 2, 5):

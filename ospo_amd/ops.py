@@ -5,7 +5,6 @@ in ``_lib``; there is no eager-PyTorch fallback on this path.
 """
 from __future__ import annotations
 
-import contextlib
 import functools
 import math
 from typing import Optional
@@ -956,46 +955,54 @@ def rotary_tables(n_pos: int, rot_dim: int, theta: float, device, scaling: Optio
     return (a.cos() * mag).float(), (a.sin() * mag).float()
 
 
-def _rows3(t: torch.Tensor, name: str, dtype, n: int, d: int) -> tuple:
-    """Strides (token, head) of a [n, heads, d] tensor."""
+_F32, _I32, _PAGED_TYPES = torch.float32, torch.int32, (torch.bfloat16, torch.float16)
+
+
+def _heads(t: torch.Tensor, name: str, dtype, n: int, d: int) -> tuple:
+    """(heads, token stride, head stride) of a [n, heads, d] tensor."""
     sh, st = t.shape, t.stride()
-    if len(sh) != 3 or sh[0] != n or sh[2] != d or (st[2] != 1 and d > 1):
-        raise ValueError(f"{name}: expected [{n}, heads, {d}] with a contiguous last dimension, got {tuple(sh)} "
-                         f"strides {st}")
-    if t.dtype != dtype:
-        raise ValueError(f"{name}: expected {dtype}, got {t.dtype}")
-    return st[0], st[1]
+    if len(sh) != 3 or sh[0] != n or sh[2] != d or (st[2] != 1 and d > 1) or t.dtype != dtype:
+        raise ValueError(f"{name}: expected {dtype} [{n}, heads, {d}] with a contiguous last dimension, got {t.dtype} "
+                         f"{tuple(sh)} strides {st}")
+    return sh[1], st[0], st[1]
 
 
-def _ints(t: torch.Tensor, name: str, *shape) -> None:
-    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+def _ints(t: torch.Tensor, name: str, shape: tuple) -> None:
+    if t.dtype != _I32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name}: expected a contiguous int32 tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
 
 
 def _rot_tables(tables, who: str) -> tuple:
+    """(cos, sin, positions, rot_dim) of rotary tables."""
     cos, sin = tables
-    if (cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or cos.shape != sin.shape
-            or not cos.is_contiguous() or not sin.is_contiguous() or cos.numel() == 0):
+    sh = cos.shape
+    if (cos.dtype != _F32 or sin.dtype != _F32 or len(sh) != 2 or sin.shape != sh or not cos.is_contiguous()
+            or not sin.is_contiguous() or 0 in sh):
         raise ValueError(f"{who}: tables are two contiguous fp32 [positions, rot_dim / 2] tensors")
-    return cos, sin
+    return cos, sin, sh[0], 2 * sh[1]
 
 
-def _one_device(who: str, *tensors) -> torch.device:
-    """The device of all tensors; refuses host tensors and a mix."""
-    dev = tensors[0].device
+def _place(who: str, *tensors) -> int:
+    """The index of the device that holds all tensors (None among them aside); refuses host tensors and a mix."""
+    i = tensors[0].get_device()
     for t in tensors:
-        if not t.is_cuda:
-            raise ValueError(f"{who}: expected device tensors")
-        if t.device != dev:
-            raise ValueError(f"{who}: tensors on {dev} and {t.device}")
-    return dev
+        if t is not None and t.get_device() != i:
+            raise ValueError(f"{who}: tensors on several devices")
+    if i < 0:
+        raise ValueError(f"{who}: expected device tensors")
+    return i
 
 
-def _on(dev: torch.device):
-    """The context that makes ``dev`` current (nothing where it is)."""
-    if dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
+def _launch(index: int, name: str, *args) -> None:
+    """call(name, *args, stream) on device ``index`` and its current stream."""
+    fn = getattr(_lib.lib(), name)
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(name, rc)
 
 
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, tables: tuple, *,
@@ -1006,39 +1013,38 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
     fp32 arithmetic, rounded once to q's type (bf16, fp16, fp32).  ``backward``: q and k are the gradients of the
     outputs, the result those of the inputs.  ``out`` (q', k'): where to write, the inputs themselves allowed; new
     tensors by default.  Returns (q', k')."""
-    cos, sin = _rot_tables(tables, "rotary")
-    if q.dim() != 3 or q.dtype not in _CODE:
-        raise ValueError(f"rotary: expected q [n, heads, head_dim] in bf16, fp16 or fp32, got {q.dtype} "
-                         f"{tuple(q.shape)}")
-    n, hq, d = q.shape
-    rot = 2 * cos.shape[1]
+    cos, sin, n_pos, rot = _rot_tables(tables, "rotary")
+    dt = q.dtype
+    code = _CODE.get(dt)
+    if q.dim() != 3 or code is None:
+        raise ValueError(f"rotary: expected q [n, heads, head_dim] in bf16, fp16 or fp32, got {dt} {tuple(q.shape)}")
+    n, _, d = q.shape
+    hq, q0, q1 = _heads(q, "q", dt, n, d)
     if hq < 1 or not 1 <= d <= 256 or rot > d:
         raise ValueError(f"rotary: {hq} heads of {d} (at most 256), of which {rot} turn")
-    qs = _rows3(q, "q", q.dtype, n, d)
-    _ints(positions, "positions", n)
-    hk, ks = 0, (0, 0)
-    if k is not None:
-        ks = _rows3(k, "k", q.dtype, n, d)
-        hk = k.shape[1]
+    _ints(positions, "positions", (n,))
     if out is None:
-        qo = torch.empty((n, hq, d), dtype=q.dtype, device=q.device)
-        ko = None if k is None else torch.empty((n, hk, d), dtype=q.dtype, device=q.device)
+        qo, ko = q.new_empty(q.shape), None if k is None else k.new_empty(k.shape)
     else:
         qo, ko = out
         if qo.shape != q.shape or (ko is None) != (k is None) or (k is not None and ko.shape != k.shape):
             raise ValueError("rotary: out has other shapes than q and k")
-    qos = _rows3(qo, "out[0]", q.dtype, n, d)
-    kos = (0, 0) if ko is None else _rows3(ko, "out[1]", q.dtype, n, d)
-    dev = _one_device("rotary", q, positions, cos, sin, qo, *(() if k is None else (k, ko)))
-    with _on(dev):
-        call("ospo_rotary", _p(q), qs[0], qs[1], _p(qo), qos[0], qos[1], hq, _p(k), ks[0], ks[1], _p(ko), kos[0],
-             kos[1], hk, n, d, rot, int(interleaved), _p(positions), _p(cos), _p(sin), cos.shape[0], int(backward),
-             _CODE[q.dtype], _s())
+    _, qo0, qo1 = _heads(qo, "out[0]", dt, n, d)
+    if k is None:
+        hk = k0 = k1 = ko0 = ko1 = 0
+        kp = kop = None
+    else:
+        hk, k0, k1 = _heads(k, "k", dt, n, d)
+        _, ko0, ko1 = _heads(ko, "out[1]", dt, n, d)
+        kp, kop = k.data_ptr(), ko.data_ptr()
+    _launch(_place("rotary", q, positions, cos, sin, qo, k, ko), "ospo_rotary", q.data_ptr(), q0, q1, qo.data_ptr(),
+            qo0, qo1, hq, kp, k0, k1, kop, ko0, ko1, hk, n, d, rot, interleaved, positions.data_ptr(), cos.data_ptr(),
+            sin.data_ptr(), n_pos, backward, code)
     return qo, ko
 
 
 def _paged(who: str, k_cache, v_cache, block_table, q_start, kv_len, dtype, d: int) -> tuple:
-    """(kv heads, n_pages, page_size, sequences, max_pages, strides) of a paged cache and its tables."""
+    """(pages, kv heads, page size, sequences, pages a sequence, strides) of a paged cache and its tables."""
     sh, st = k_cache.shape, k_cache.stride()
     if len(sh) != 4 or sh[3] != d or (st[3] != 1 and d > 1) or k_cache.dtype != dtype:
         raise ValueError(f"{who}: expected {dtype} caches [pages, kv_heads, page_size, {d}] with a contiguous last "
@@ -1047,13 +1053,13 @@ def _paged(who: str, k_cache, v_cache, block_table, q_start, kv_len, dtype, d: i
         raise ValueError(f"{who}: k_cache and v_cache differ in shape, type or strides")
     if sh[1] < 1 or sh[2] < 1:
         raise ValueError(f"{who}: empty heads or pages in a cache of shape {tuple(sh)}")
-    if block_table.dim() != 2:
+    bt = block_table.shape
+    if len(bt) != 2:
         raise ValueError(f"{who}: block_table is int32 [sequences, pages]")
-    n_seqs, max_pages = block_table.shape
-    _ints(block_table, "block_table", n_seqs, max_pages)
-    _ints(q_start, "q_start", n_seqs + 1)
-    _ints(kv_len, "kv_len", n_seqs)
-    return sh[1], sh[0], sh[2], n_seqs, max_pages, st
+    _ints(block_table, "block_table", bt)
+    _ints(q_start, "q_start", (bt[0] + 1,))
+    _ints(kv_len, "kv_len", (bt[0],))
+    return sh[0], sh[1], sh[2], bt[0], bt[1], st
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -1066,50 +1072,51 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     tokens, kv_len[s] its length with them, block_table[s] its pages (all int32, read on the device).  With ``q``
     [n, q_heads, head_dim] its turned copy is returned (``q_out``; may be q itself).  Rows of no sequence are left
     alone; a row whose position or page does not exist is not stored."""
-    if k.dim() != 3 or k.dtype not in _CODE:
-        raise ValueError(f"paged_append: expected k [n, kv_heads, head_dim] in bf16, fp16 or fp32, got {k.dtype} "
-                         f"{tuple(k.shape)}")
-    n, hk, d = k.shape
     dt = k.dtype
-    ks, vs = _rows3(k, "k", dt, n, d), _rows3(v, "v", dt, n, d)
-    heads, n_pages, page, n_seqs, max_pages, st = _paged("paged_append", k_cache, v_cache, block_table, q_start, kv_len,
+    code = _CODE.get(dt)
+    if k.dim() != 3 or code is None:
+        raise ValueError(f"paged_append: expected k [n, kv_heads, head_dim] in bf16, fp16 or fp32, got {dt} "
+                         f"{tuple(k.shape)}")
+    n, _, d = k.shape
+    hk, k0, k1 = _heads(k, "k", dt, n, d)
+    hv, v0, v1 = _heads(v, "v", dt, n, d)
+    n_pages, heads, page, n_seqs, max_pages, st = _paged("paged_append", k_cache, v_cache, block_table, q_start, kv_len,
                                                          dt, d)
-    if v.shape[1] != hk or heads != hk:
-        raise ValueError(f"paged_append: {hk} heads in k, {v.shape[1]} in v, {heads} in the cache")
+    if hv != hk or heads != hk:
+        raise ValueError(f"paged_append: {hk} heads in k, {hv} in v, {heads} in the cache")
     if not 1 <= d <= 256:
         raise ValueError(f"paged_append: head_dim {d} outside [1, 256]")
-    if rope is None:
-        cos = sin = None
-        rot = n_pos = 0
-    else:
-        cos, sin = _rot_tables(rope, "paged_append")
-        n_pos, rot = cos.shape[0], 2 * cos.shape[1]
+    cos = sin = cp = sp = None
+    rot = n_pos = 0
+    if rope is not None:
+        cos, sin, n_pos, rot = _rot_tables(rope, "paged_append")
+        cp, sp = cos.data_ptr(), sin.data_ptr()
         if rot > d:
             raise ValueError(f"paged_append: {rot} of {d} elements turn")
-    hq, qs, qos = 0, (0, 0), (0, 0)
+    hq = q0 = q1 = qo0 = qo1 = 0
+    qp = qop = None
     if q is not None:
-        qs, hq = _rows3(q, "q", dt, n, d), q.shape[1]
+        hq, q0, q1 = _heads(q, "q", dt, n, d)
         if q_out is None:
-            q_out = torch.empty((n, hq, d), dtype=dt, device=q.device)
+            q_out = q.new_empty(q.shape)
         elif q_out.shape != q.shape:
             raise ValueError("paged_append: q_out has another shape than q")
-        qos = _rows3(q_out, "q_out", dt, n, d)
+        _, qo0, qo1 = _heads(q_out, "q_out", dt, n, d)
+        qp, qop = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("paged_append: q_out without q")
-    dev = _one_device("paged_append", k, v, k_cache, v_cache, block_table, q_start, kv_len,
-                      *(() if q is None else (q, q_out)), *(() if rope is None else (cos, sin)))
-    with _on(dev):
-        call("ospo_paged_append", _p(k), ks[0], ks[1], _p(v), vs[0], vs[1], _p(q), qs[0], qs[1], _p(q_out), qos[0],
-             qos[1], n, hq, hk, d, _p(k_cache), _p(v_cache), st[0], st[1], st[2], n_pages, page, _p(block_table),
-             max_pages, _p(q_start), _p(kv_len), n_seqs, _p(cos), _p(sin), n_pos, rot, int(interleaved), _CODE[dt],
-             _s())
+    _launch(_place("paged_append", k, v, k_cache, v_cache, block_table, q_start, kv_len, q, q_out, cos, sin),
+            "ospo_paged_append", k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, qp, q0, q1, qop, qo0, qo1, n, hq, hk, d,
+            k_cache.data_ptr(), v_cache.data_ptr(), st[0], st[1], st[2], n_pages, page, block_table.data_ptr(),
+            max_pages, q_start.data_ptr(), kv_len.data_ptr(), n_seqs, cp, sp, n_pos, rot, interleaved, code)
     return q_out
 
 
 @functools.lru_cache(maxsize=4096)
 def _paged_attn_ws_bytes(index: int, *shape) -> int:
-    """ospo_paged_attn_ws_bytes on the current device ``index``."""
-    return int(query("ospo_paged_attn_ws_bytes", *shape))
+    """ospo_paged_attn_ws_bytes on device ``index``."""
+    with torch.cuda.device(index):
+        return int(query("ospo_paged_attn_ws_bytes", *shape))
 
 
 def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -1122,40 +1129,43 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
     h // (q_heads // kv_heads).  One call takes chunks and single tokens together.  Returns out [n, q_heads,
     head_dim]; lse (fp32 [n, q_heads], optional) gets the natural log of each row's sum of exponentials.  A row that
     sees nothing is zero, its lse -inf; rows of no sequence are left as they were (in a new ``out``: anything)."""
-    if q.dim() != 3 or q.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"paged_attn: expected q [n, heads, head_dim] in bf16 or fp16, got {q.dtype} {tuple(q.shape)}")
-    n, hq, d = q.shape
     dt = q.dtype
+    if q.dim() != 3 or dt not in _PAGED_TYPES:
+        raise ValueError(f"paged_attn: expected q [n, heads, head_dim] in bf16 or fp16, got {dt} {tuple(q.shape)}")
+    n, _, d = q.shape
     if d not in (64, 128, 256):
         raise ValueError(f"paged_attn: head_dim {d} not in (64, 128, 256)")
     scale = float(scale)
     if not 0.0 < scale < math.inf:
         raise ValueError(f"paged_attn: scale {scale} (positive and finite)")
-    qs = _rows3(q, "q", dt, n, d)
-    hk, n_pages, page, n_seqs, max_pages, st = _paged("paged_attn", k_cache, v_cache, block_table, q_start, kv_len, dt, d)
+    hq, q0, q1 = _heads(q, "q", dt, n, d)
+    n_pages, hk, page, n_seqs, max_pages, st = _paged("paged_attn", k_cache, v_cache, block_table, q_start, kv_len, dt, d)
     if hq < 1 or hq % hk:
         raise ValueError(f"paged_attn: {hq} query heads over {hk} key/value heads")
     if st[0] % 8 or st[1] % 8 or st[2] % 8:
         raise ValueError(f"paged_attn: cache strides {st} are not multiples of 8")
+    sp = None
     if start is not None:
-        _ints(start, "start", n_seqs)
+        _ints(start, "start", (n_seqs,))
+        sp = start.data_ptr()
     if out is None:
-        out = torch.empty((n, hq, d), dtype=dt, device=q.device)
+        out = q.new_empty(q.shape)
     elif out.shape != q.shape:
         raise ValueError("paged_attn: out has another shape than q")
-    os_ = _rows3(out, "out", dt, n, d)
-    ls = (0, 0)
+    _, o0, o1 = _heads(out, "out", dt, n, d)
+    l0 = l1 = 0
+    lp = None
     if lse is not None:
-        if lse.dtype != torch.float32 or lse.shape != (n, hq):
+        if lse.dtype != _F32 or lse.shape != (n, hq):
             raise ValueError(f"paged_attn: lse is fp32 [{n}, {hq}], got {lse.dtype} {tuple(lse.shape)}")
-        ls = lse.stride()
-    dev = _one_device("paged_attn", q, k_cache, v_cache, block_table, q_start, kv_len, out,
-                      *(() if start is None else (start,)), *(() if lse is None else (lse,)))
-    with _on(dev):
-        nbytes = _paged_attn_ws_bytes(dev.index, n, n_seqs, hq, hk, d, page, max_pages)
-        # a workspace of its own for each call: freed in stream order, and held by the graph that captures the call
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        call("ospo_paged_attn", _p(q), qs[0], qs[1], _p(k_cache), _p(v_cache), st[0], st[1], st[2], n_pages, page,
-             _p(block_table), max_pages, _p(q_start), _p(kv_len), _p(start), n_seqs, n, hq, hk, d, scale, int(causal),
-             _p(out), os_[0], os_[1], _p(lse), ls[0], ls[1], _CODE[dt], _p(ws), nbytes, _s())
+        l0, l1 = lse.stride()
+        lp = lse.data_ptr()
+    index = _place("paged_attn", q, k_cache, v_cache, block_table, q_start, kv_len, out, start, lse)
+    nbytes = _paged_attn_ws_bytes(index, n, n_seqs, hq, hk, d, page, max_pages)
+    # a workspace of its own for each call: freed in stream order, and held by the graph that captures the call
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _launch(index, "ospo_paged_attn", q.data_ptr(), q0, q1, k_cache.data_ptr(), v_cache.data_ptr(), st[0], st[1], st[2],
+            n_pages, page, block_table.data_ptr(), max_pages, q_start.data_ptr(), kv_len.data_ptr(), sp, n_seqs, n, hq,
+            hk, d, scale, causal, out.data_ptr(), o0, o1, lp, l0, l1, _CODE[dt], None if ws is None else ws.data_ptr(),
+            nbytes)
     return out
