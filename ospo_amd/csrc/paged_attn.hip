@@ -48,125 +48,134 @@ struct PagedArgs {
 };
 
 // ---------------------------------------------------------------- items
+// Wave-wide sums by data-parallel moves: rows of 16 lanes, then across the rows (a lane without a source adds 0).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp0(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int scan_add(int x) {  // inclusive
+  x += dpp0<0x111, 0xf>(x);
+  x += dpp0<0x112, 0xf>(x);
+  x += dpp0<0x114, 0xf>(x);
+  x += dpp0<0x118, 0xf>(x);
+  x += dpp0<0x142, 0xa>(x);
+  x += dpp0<0x143, 0xc>(x);
+  return x;
+}
+__device__ __forceinline__ int lane_of(int x, int l) { return __builtin_amdgcn_readlane(x, l); }
+__device__ __forceinline__ int sum_i(int x) { return lane_of(scan_add(x), 63); }
+__device__ __forceinline__ float sum_f(float x) {
+#define OSPO_STEP(C, R) x += __int_as_float(dpp0<C, R>(__float_as_int(x)))
+  OSPO_STEP(0x111, 0xf);
+  OSPO_STEP(0x112, 0xf);
+  OSPO_STEP(0x114, 0xf);
+  OSPO_STEP(0x118, 0xf);
+  OSPO_STEP(0x142, 0xa);
+  OSPO_STEP(0x143, 0xc);
+#undef OSPO_STEP
+  return __int_as_float(lane_of(__float_as_int(x), 63));
+}
+__device__ __forceinline__ int max_i(int x) {  // of values >= 0
+  x = max(x, dpp0<0x111, 0xf>(x));
+  x = max(x, dpp0<0x112, 0xf>(x));
+  x = max(x, dpp0<0x114, 0xf>(x));
+  x = max(x, dpp0<0x118, 0xf>(x));
+  x = max(x, dpp0<0x142, 0xa>(x));
+  x = max(x, dpp0<0x143, 0xc>(x));
+  return lane_of(x, 63);
+}
+
+struct LaneSeq {  // the sequence of this lane: its rows in tiles of BM, its keys in units of KU
+  Seq q;
+  int tiles, units;
+};
 // units: key blocks of KU that the sequence's longest row sees (every tile of it is cut at the same places)
-__device__ __forceinline__ void seq_tiles(const Seq& q, const FDiv& g, int BM, int KU, int& tiles, int& units) {
-  const long r = (long)q.n * (int)g.d;
-  tiles = (int)((r + BM - 1) / BM);
-  units = q.kv > q.st ? (q.kv + KU - 1) / KU - q.st / KU : 0;
-  if (units < 1) units = 1;
-}
-__device__ __forceinline__ long wave_sum_l(long v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
-__device__ __forceinline__ int wave_max_i(int v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
-  return v;
+template <int BM, int KU>
+__device__ __forceinline__ LaneSeq lane_seq(const PagedArgs& a, int s) {
+  LaneSeq r{{0, 0, 0, 0}, 0, 1};
+  if (s < a.S) {
+    r.q = load_seq(a.qs, a.kl, a.st, s, a.rows, a.most);
+    r.tiles = (r.q.n * (int)a.g.d + BM - 1) / BM;
+    r.units = r.q.kv > r.q.st ? (r.q.kv + KU - 1) / KU - r.q.st / KU : 1;
+  }
+  return r;
 }
 // Key blocks of a chunk.  With L = all work / slots: where the tiles alone fill the slots, chunks of at most L / 4
-// even out the last round (only the long sequences are cut once there are many tiles); where they do not, the
-// smallest chunk that keeps one round.
-__device__ int pick_chunk(const PagedArgs& a, int lane, int BM, int KU) {
-  long total = 0, base = 0;
-  int most = 1;
+// even out the last round (with many tiles, only sequences longer than L are cut); where they do not, the smallest
+// chunk that keeps one round.
+template <int BM, int KU>
+__device__ __forceinline__ int pick_chunk(const PagedArgs& a, int lane, const LaneSeq& first) {
+  if (!a.split) return 0x7fffffff;
+  float total = 0.f;
+  int base = 0, most = 1;
   for (int s0 = 0; s0 < a.S; s0 += 64) {
-    const int s = s0 + lane;
-    if (s < a.S) {
-      const Seq q = load_seq(a.qs, a.kl, a.st, s, a.rows, a.most);
-      int t, u;
-      seq_tiles(q, a.g, BM, KU, t, u);
-      if (t) most = max(most, u);
-      total += (long)t * u;
-      base += t;
-    }
+    const LaneSeq q = s0 ? lane_seq<BM, KU>(a, s0 + lane) : first;
+    total += sum_f((float)q.tiles * (float)q.units);
+    base += sum_i(q.tiles);
+    most = max(most, max_i(q.tiles ? q.units : 0));
   }
-  total = wave_sum_l(total) * a.Hk;
-  base = wave_sum_l(base) * a.Hk;
-  most = wave_max_i(most);
-  if (!a.split) return most;
-  const long L = (total + a.slots - 1) / a.slots;
-  if (base > a.slots) {
-    const long c = base >= 4l * a.slots ? L : (L + 3) / 4;
-    return (int)min((long)most, max(1l, c));
-  }
-  int C = (int)min((long)most, max(1l, L));
+  base *= a.Hk;
+  const float L = total * (float)a.Hk / (float)a.slots;
+  if (base > a.slots) return (int)fminf((float)most, ceilf(base >= 4 * a.slots ? L : 0.25f * L));
+  int C = (int)fminf((float)most, fmaxf(1.f, ceilf(L)));
   while (C < most) {
-    long n = 0;
+    int n = 0;
     for (int s0 = 0; s0 < a.S; s0 += 64) {
-      const int s = s0 + lane;
-      if (s < a.S) {
-        const Seq q = load_seq(a.qs, a.kl, a.st, s, a.rows, a.most);
-        int t, u;
-        seq_tiles(q, a.g, BM, KU, t, u);
-        n += (long)t * ((u + C - 1) / C);
-      }
+      const LaneSeq q = s0 ? lane_seq<BM, KU>(a, s0 + lane) : first;
+      n += sum_i(q.tiles * (int)(((unsigned)q.units + C - 1) / (unsigned)C));
     }
-    if (wave_sum_l(n) * a.Hk <= a.slots) break;
+    if (n * a.Hk <= a.slots) break;
     C += (C + 7) / 8;
   }
-  return min(C, most);
+  return C;
 }
 
 struct Item {
   Seq q;
   int seq, tile, head, chunk, nch, cs, u0, units;
-  long first;  // item index of chunk 0 of this (tile, head); chunks are `step` apart
-  int step;
+  int first, step;  // item index of chunk 0 of this (tile, head); its chunks are `step` apart
 };
 // Order of a sequence's items: heads fastest over the XCDs (hb = largest power of two <= 8 that divides Hk, so a
-// key/value head stays on its XCDs' L2), then chunks, then tiles from the last (the longest rows first), then the
-// remaining heads.
-// mode 0: find the item; mode 1: find (tile, head) pair number `id` (the joining launch)
-__device__ bool find_item(const PagedArgs& a, long id, int lane, int BM, int KU, int mode, Item& it) {
-  const int C = pick_chunk(a, lane, BM, KU);
-  long before = 0, ibefore = 0;
+// key/value head stays in its XCDs' L2), then chunks, then tiles from the last (the longest rows first), then the
+// remaining heads.  PAIR: item number `id` counts (tile, head) pairs (the joining launch).
+template <int BM, int KU, bool PAIR>
+__device__ __forceinline__ bool find_item(const PagedArgs& a, int id, int lane, Item& it) {
+  const LaneSeq lead = lane_seq<BM, KU>(a, lane);
+  const unsigned C = (unsigned)max(1, pick_chunk<BM, KU>(a, lane, lead));
+  int before = 0, ibefore = 0;
   for (int s0 = 0; s0 < a.S; s0 += 64) {
-    const int s = s0 + lane;
-    Seq q{0, 0, 0, 0};
-    int t = 0, u = 1, nch = 1;
-    if (s < a.S) {
-      q = load_seq(a.qs, a.kl, a.st, s, a.rows, a.most);
-      seq_tiles(q, a.g, BM, KU, t, u);
-      nch = (u + C - 1) / C;
-    }
-    const long mine = (long)t * a.Hk * (mode ? 1 : nch);
-    long inc = mine, iinc = (long)t * a.Hk * nch;
-    const long imine = iinc;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const long x = __shfl_up(inc, o, 64), y = __shfl_up(iinc, o, 64);
-      if (lane >= o) inc += x, iinc += y;
-    }
-    const bool here = id >= before + inc - mine && id < before + inc;
-    const unsigned long long b = __ballot(here);
+    const LaneSeq q = s0 ? lane_seq<BM, KU>(a, s0 + lane) : lead;
+    const int nch = (int)(((unsigned)q.units - 1) / C) + 1;
+    const int pairs = q.tiles * a.Hk;
+    const int items = scan_add(pairs * nch);
+    const int mine = PAIR ? scan_add(pairs) : items;
+    const unsigned long long b = __ballot(id - before < mine);
     if (b) {
       const int w = __ffsll(b) - 1;
-      it.q.q0 = __shfl(q.q0, w, 64), it.q.n = __shfl(q.n, w, 64);
-      it.q.kv = __shfl(q.kv, w, 64), it.q.st = __shfl(q.st, w, 64);
       it.seq = s0 + w;
-      const int tiles = __shfl(t, w, 64);
-      it.units = __shfl(u, w, 64), it.nch = __shfl(nch, w, 64);
-      const long at = id - before - __shfl(inc - mine, w, 64);
-      const long ibase = ibefore + __shfl(iinc - imine, w, 64);
-      int hb = 8;
-      while (a.Hk % hb) hb >>= 1;
-      const int per = mode ? tiles : tiles * it.nch;
-      const int hl = (int)(at % hb);
-      const long z = at / hb;
-      const int hh = (int)(z / per), x = (int)(z % per);
-      it.head = hh * hb + hl;
-      it.tile = tiles - 1 - (mode ? x : x / it.nch);
-      it.chunk = mode ? 0 : x % it.nch;
-      it.cs = (it.units + it.nch - 1) / it.nch;
+      it.q.q0 = lane_of(q.q.q0, w), it.q.n = lane_of(q.q.n, w);
+      it.q.kv = lane_of(q.q.kv, w), it.q.st = lane_of(q.q.st, w);
+      it.units = lane_of(q.units, w), it.nch = lane_of(nch, w);
+      const unsigned tiles = (unsigned)lane_of(q.tiles, w);
+      const int np = lane_of(pairs, w);
+      const unsigned at = (unsigned)(id - before - (lane_of(mine, w) - (PAIR ? np : np * it.nch)));
+      const int ibase = ibefore + lane_of(items, w) - np * it.nch;
+      const int hb = min(8, a.Hk & -a.Hk), sh = __ffs(hb) - 1;
+      const unsigned hl = at & (hb - 1), z = at >> sh;
+      const unsigned per = PAIR ? tiles : tiles * it.nch;
+      const unsigned hh = z / per, x = z - hh * per;
+      const unsigned tx = PAIR ? x : x / it.nch;
+      it.head = (int)(hh * hb + hl);
+      it.tile = (int)(tiles - 1 - tx);
+      it.chunk = PAIR ? 0 : (int)(x - tx * it.nch);
+      it.cs = (int)(((unsigned)it.units + it.nch - 1) / it.nch);
       it.u0 = it.q.st / KU;
-      it.first = ibase + ((long)hh * tiles * it.nch + (long)(tiles - 1 - it.tile) * it.nch) * hb + hl;
+      it.first = ibase + (int)(((hh * tiles + tx) * it.nch << sh) + hl);
       it.step = hb;
       return true;
     }
-    before += __shfl(inc, 63, 64);
-    ibefore += __shfl(iinc, 63, 64);
+    before += lane_of(mine, 63);
+    ibefore += lane_of(items, 63);
   }
   return false;
 }
@@ -196,6 +205,21 @@ struct Frag<f16> {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0);
   }
 };
+
+// A fragment of values as finite numbers (others as zeros), and where +infinity and -infinity (NaN: both) stand
+template <typename T>
+__device__ __forceinline__ void split_values(const i16x8& v, typename Frag<T>::v8& fin, typename Frag<T>::v8& up,
+                                             typename Frag<T>::v8& dn) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const short e = v[i];  // (a copy: a bit cast of the vector's element itself takes element 0)
+    const unsigned bits = (unsigned short)e;
+    const bool odd = (bits & Frag<T>::EXP) == Frag<T>::EXP, nan = odd && (bits & Frag<T>::MAN);
+    fin[i] = odd ? (T)0.f : __builtin_bit_cast(T, e);
+    up[i] = nan || (odd && !(bits & 0x8000)) ? (T)1.f : (T)0.f;
+    dn[i] = nan || (odd && (bits & 0x8000)) ? (T)1.f : (T)0.f;
+  }
+}
 
 // LDS images are [key][D] with the 16-byte chunks of a row swizzled so that both the row reads of K (32 rows, one
 // chunk) and the transposed reads of V (4 rows x 4 chunks) meet every bank once: 256-byte rows rotate by
@@ -265,7 +289,7 @@ __global__ __launch_bounds__(64 * WR * WK) void paged_attn_kernel(const PagedArg
   const int hi = lane >> 5, l32 = lane & 31;
 
   Item it;
-  if (!find_item(a, blockIdx.x, lane, BM, KU, 0, it)) return;
+  if (!find_item<BM, KU, false>(a, blockIdx.x, lane, it)) return;
   const int R = it.q.n * (int)a.g.d;  // rows of the sequence
   const int ub = it.u0 + it.chunk * it.cs;
   const int kb = ub * KU;  // the chunk's keys: kb (a multiple of KU) .. ke - 1
@@ -427,14 +451,9 @@ __global__ __launch_bounds__(64 * WR * WK) void paged_attn_kernel(const PagedArg
               const i16x8 v = vfrag(c, u);
               v8 fin, isup, isdn, seen;
               const v8 pu = u == 0 ? pt[0] : u == 1 ? pt[1] : KT > 32 && u == 2 ? pt[KT > 32 ? 2 : 0] : pt[KT > 32 ? 3 : 1];
+split_values<T>(v, fin, isup, isdn);
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                const short e = v[i];  // (a copy: a bit cast of the vector's element itself takes element 0)
-                const unsigned bits = (unsigned short)e;
-                const bool odd = (bits & F::EXP) == F::EXP, nan = odd && (bits & F::MAN);
-                fin[i] = odd ? (T)0.f : __builtin_bit_cast(T, e);
-                isup[i] = nan || (odd && !(bits & 0x8000)) ? (T)1.f : (T)0.f;
-                isdn[i] = nan || (odd && (bits & 0x8000)) ? (T)1.f : (T)0.f;
                 const int key = k0 + 16 * u + 4 * hi + (i & 3) + 8 * (i >> 2);
                 seen[i] = key > lim[b] || key < it.q.st ? (T)0.f : (T)1.f;
               }
@@ -511,12 +530,333 @@ __global__ __launch_bounds__(64 * WR * WK) void paged_attn_kernel(const PagedArg
   }
 }
 
+// ---------------------------------------------------------------- few rows
+// Up to 16 rows for each sequence and key/value head (single tokens): the keys' bytes bound it.  Four waves share out
+// the key tiles (32 keys each); a wave streams on its own, with no barrier until the end: while it works on a tile,
+// the next one's keys are on their way into registers (they are the A operand of S^T = K Q^T as they lie in
+// memory) and its values into LDS (from where the transposed reads of O^T += V^T P^T take them).  16 x 16 x 32
+// products: a 32-row form would spend twice the exponentials and registers on rows that are not there.
+//
+// The V image of 16 keys x 32 columns is 1 KiB: [16-byte chunk q][key ^ 8 (q & 1)], so that the transposed reads of
+// half a wave (8 keys x 2 chunks) meet every bank once.
+template <typename T>
+struct Mma16;
+template <>
+struct Mma16<bf16> {
+  __device__ static f32x4 mma(const bf16x8& x, const bf16x8& y, const f32x4& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma16<f16> {
+  __device__ static f32x4 mma(const f16x8& x, const f16x8& y, const f32x4& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0);
+  }
+};
+
+// value of every lane combined with those 16, 32 and 48 lanes on
+__device__ __forceinline__ float max_groups(float x) {
+  unsigned u = __float_as_uint(x);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  u = __float_as_uint(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+  const auto q = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+}
+__device__ __forceinline__ float sum_groups(float x) {
+  unsigned u = __float_as_uint(x);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  u = __float_as_uint(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+  const auto q = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __uint_as_float(q[0]) + __uint_as_float(q[1]);
+}
+
+// 4 chains (64 columns) of V^T fragments: 8 transposed reads and their wait in one block, so that no read is in
+// flight outside it (the compiler would also drain the LDS-DMA of the next tile in front of reads that it sees)
+template <int OFF, int HI>
+__device__ __forceinline__ void read_v4(unsigned at, i16x4 (&lo)[4], i16x4 (&hi)[4]) {
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8 offset:%9\n\t"
+      "ds_read_b64_tr_b16 %1, %8 offset:%10\n\t"
+      "ds_read_b64_tr_b16 %2, %8 offset:%11\n\t"
+      "ds_read_b64_tr_b16 %3, %8 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %4, %8 offset:%13\n\t"
+      "ds_read_b64_tr_b16 %5, %8 offset:%14\n\t"
+      "ds_read_b64_tr_b16 %6, %8 offset:%15\n\t"
+      "ds_read_b64_tr_b16 %7, %8 offset:%16\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(lo[0]), "=&v"(lo[1]), "=&v"(lo[2]), "=&v"(lo[3]), "=&v"(hi[0]), "=&v"(hi[1]), "=&v"(hi[2]), "=&v"(hi[3])
+      : "v"(at), "n"(OFF), "n"(OFF + 512), "n"(OFF + 1024), "n"(OFF + 1536), "n"(OFF + HI), "n"(OFF + HI + 512),
+        "n"(OFF + HI + 1024), "n"(OFF + HI + 1536)
+      : "memory");
+}
+
+template <typename T, int D, bool P16>
+__global__ __launch_bounds__(256) void paged_few_kernel(const PagedArgs a) {
+  using v8 = typename Frag<T>::v8;
+  constexpr int BM = 16, KT = 32, NW = 4, KU = KT * NW;
+  constexpr int KS = D / 32;   // d steps of S; also 64-byte column blocks of a row
+  constexpr int DC = D / 16;   // d chains of O
+  constexpr int VB = KT * D * 2;  // bytes of a V tile
+  constexpr int PITCH = pitch_of(D);
+  constexpr int OUT = NW * BM * PITCH * 4 + NW * BM * 8;
+  __shared__ __attribute__((aligned(16))) char smem[2 * NW * VB > OUT ? 2 * NW * VB : OUT];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int G = lane >> 4, l16 = lane & 15;
+
+  Item it;
+  if (!find_item<BM, KU, false>(a, blockIdx.x, lane, it)) return;
+  const int R = it.q.n * (int)a.g.d;
+  const int ub = it.u0 + it.chunk * it.cs;
+  const int kb = ub * KU;
+  const int ke = min(min(ub + it.cs, it.u0 + it.units) * KU, tile_end(a, it, BM));
+  const bool part = it.nch > 1;
+  if (part && it.chunk > 0 && kb >= ke) return;  // the joining launch counts the same chunks
+  const int row0 = it.tile * BM;
+
+  // this lane's row (rows behind the last repeat it and are not stored)
+  v8 qf[KS];
+  const int r = min(row0 + l16, R - 1);
+  const int tok = fdiv(r, a.g), hd = it.head * (int)a.g.d + r - tok * (int)a.g.d;
+  const int lim = a.causal ? it.q.kv - it.q.n + tok : it.q.kv - 1;
+  {
+    const T* p = (const T*)a.q + (long)(it.q.q0 + tok) * a.q_ts + (long)hd * a.q_hs + 8 * G;
+    if (a.qvec) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const v8*>(p + 32 * ks);
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) qf[ks][i] = p[32 * ks + i];
+    }
+  }
+  // smallest limit of the tile's rows: its first row's
+  const int low = a.causal ? it.q.kv - it.q.n + fdiv(row0, a.g) : it.q.kv - 1;
+
+  f32x4 o[DC];
+#pragma unroll
+  for (int c = 0; c < DC; ++c) o[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = NONE, l = 0.f;
+
+  // addresses: pages are read ahead of their keys
+  const T* kc = (const T*)a.kc + (long)it.head * a.c_hs;
+  const T* vc = (const T*)a.vc + (long)it.head * a.c_hs;
+  const int* bt = a.bt + (long)it.seq * a.max_pages;
+  const int n = ke > kb + wave * KT ? (ke - kb - wave * KT + KU - 1) / KU : 0;  // this wave's tiles
+  const int kw = kb + wave * KT;  // its first key
+  const int lastp = ke > 0 ? fdiv(ke - 1, a.ps) : 0;
+  const int vrow = l16 ^ ((G & 1) << 3);  // key of this lane in a V piece
+  char* vbuf = smem + wave * VB;
+  auto clampp = [&](int p) __attribute__((always_inline)) { return min(max(p, 0), a.n_pages - 1); };
+
+  // P16 (the page size is a multiple of 16): 16 keys lie in one page; 64 page numbers at a time sit on the lanes.
+  // Slots behind a sequence's end are read (they are inside its last page) and masked.
+  int pbase = 0, pv = 0, pn = 0;
+  // otherwise every lane looks up its own rows, one tile ahead: K rows l16 and 16 + l16, V rows vrow and 16 + vrow
+  int pg[4];
+  auto lookup = [&](int k0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int key = min(k0 + (i & 1) * 16 + (i < 2 ? l16 : vrow), ke - 1);
+      pg[i] = bt[fdiv(key, a.ps)];
+    }
+  };
+  if (n > 0) {
+    if constexpr (P16) {
+      pbase = fdiv(kw, a.ps);
+      pv = clampp(bt[min(pbase + lane, lastp)]);
+      pn = bt[min(pbase + 64 + lane, lastp)];
+    } else {
+      lookup(kw);
+    }
+  }
+
+  // start tile i: V into LDS buffer `buf`, K into registers
+  auto issue = [&](int i, char* buf, v8 (&kf)[2][KS]) __attribute__((always_inline)) {
+    const int k0 = kw + i * KU;
+    const T* kp[2];
+    const T* vp[2];
+    if constexpr (P16) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int k1 = k0 + 16 * t;
+        const int pi = fdiv(k1, a.ps), slot = k1 - pi * (int)a.ps.d;
+        const int pc = min(pi, lastp);
+        if (pc - pbase >= 64) {
+          pbase += 64;
+          pv = clampp(pn);
+          pn = bt[min(pbase + 64 + lane, lastp)];
+        }
+        const long off = (long)lane_of(pv, pc - pbase) * a.c_ps + (long)slot * a.c_ts;
+        kp[t] = kc + off + l16 * a.c_ts;
+        vp[t] = vc + off + vrow * a.c_ts;
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int kk = min(k0 + 16 * t + l16, ke - 1), kv = min(k0 + 16 * t + vrow, ke - 1);
+        kp[t] = kc + (long)clampp(pg[t]) * a.c_ps + (long)(kk - fdiv(kk, a.ps) * (int)a.ps.d) * a.c_ts;
+        vp[t] = vc + (long)clampp(pg[2 + t]) * a.c_ps + (long)(kv - fdiv(kv, a.ps) * (int)a.ps.d) * a.c_ts;
+      }
+      if (i + 1 < n) lookup(k0 + KU);
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int p = 0; p < KS; ++p) dma16(vp[t] + 32 * p + 8 * G, buf + (t * KS + p) * 1024);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) kf[t][ks] = *reinterpret_cast<const v8*>(kp[t] + 32 * ks + 8 * G);
+  };
+
+  const int li = lane & 15, vq = (li & 3) >> 1;
+  const unsigned va = (unsigned)(uintptr_t)((LDS_AS const char*)vbuf) +
+                      (vq * 16 + ((4 * G + (li >> 2)) ^ (vq << 3))) * 16 + (li & 1) * 8;
+  v8 ka[2][KS], kn[2][KS];
+  auto work = [&](int i, int b, v8 (&kf)[2][KS]) __attribute__((always_inline)) {
+    const int k0 = kw + i * KU;
+    f32x4 s[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) s[t] = Mma16<T>::mma(kf[t][ks], qf[ks], s[t]);
+    }
+    const bool mask = k0 < it.q.st || k0 + KT - 1 > low;
+    if (mask) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = k0 + 16 * t + 4 * G + e;
+          s[t][e] = key > lim || key < it.q.st ? -INFINITY : s[t][e];
+        }
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[t][e]);
+    mx = max_groups(mx);
+    const float mn = fmaxf(m, mx * a.cs);
+    const float alpha = __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
+    float sum = 0.f;
+    v8 pt;  // P in the cache's type (rounded to nearest: the matrix unit's operand; the sum keeps fp32)
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[t][e], a.cs, -mn));
+        sum += p;
+        pt[4 * t + e] = (T)p;
+      }
+    l = l * alpha + sum;  // this lane's keys; the lanes of a row are added up at the end
+    const unsigned vb = va + b * NW * VB;
+#pragma unroll
+    for (int c4 = 0; c4 < DC; c4 += 4) {
+      i16x4 lo[4], hi[4];
+      // (a column block's 64 columns are 2 KiB; key group 1 lies KS KiB behind group 0)
+      if (c4 == 0) read_v4<0, KS * 1024>(vb, lo, hi);
+      if (c4 == 4) read_v4<2048, KS * 1024>(vb, lo, hi);
+      if (c4 == 8) read_v4<4096, KS * 1024>(vb, lo, hi);
+      if (c4 == 12) read_v4<6144, KS * 1024>(vb, lo, hi);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const i16x8 vv = {lo[c][0], lo[c][1], lo[c][2], lo[c][3], hi[c][0], hi[c][1], hi[c][2], hi[c][3]};
+        if (!mask) {
+          o[c4 + c] = Mma16<T>::mma(__builtin_bit_cast(v8, vv), pt, o[c4 + c] * alpha);
+        } else {
+          // a value that some row doesn't see must not reach it, whatever it is: see paged_attn_kernel
+          f32x4 x = Mma16<T>::mma(__builtin_bit_cast(v8, vv), pt, f32x4{0.f, 0.f, 0.f, 0.f});
+          float bad = 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) bad = fmaf(x[e], 0.f, bad);
+          if (__ballot(bad != 0.f)) {
+            v8 fin, up, dn, seen;
+            split_values<T>(vv, fin, up, dn);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int key = k0 + 16 * (e >> 2) + 4 * G + (e & 3);
+              seen[e] = key > lim || key < it.q.st ? (T)0.f : (T)1.f;
+            }
+            const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+            x = Mma16<T>::mma(fin, pt, z);
+            const f32x4 u = Mma16<T>::mma(up, seen, z), w = Mma16<T>::mma(dn, seen, z);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (u[e] > 0.f) x[e] += INFINITY;
+              if (w[e] > 0.f) x[e] -= INFINITY;
+            }
+          }
+          o[c4 + c] = o[c4 + c] * alpha + x;
+        }
+      }
+    }
+  };
+  // operations of one issue() behind which a wait may stop: the V pieces and K loads of the next tile
+  constexpr int AHEAD = 4 * KS;
+  auto step = [&](int i, int b, v8 (&kf)[2][KS], v8 (&kx)[2][KS]) __attribute__((always_inline)) {
+    if (i + 1 < n) {
+      issue(i + 1, vbuf + (b ^ 1) * NW * VB, kx);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(AHEAD) : "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    work(i, b, kf);
+  };
+  if (n > 0) issue(0, vbuf, ka);
+  for (int i = 0; i < n; i += 2) {
+    step(i, 0, ka, kn);
+    if (i + 1 < n) step(i + 1, 1, kn, ka);
+  }
+  l = sum_groups(l);
+
+  // join the waves and store
+  const int rows = min(BM, R - row0);
+  float* ml = reinterpret_cast<float*>(smem + NW * BM * PITCH * 4);
+  __syncthreads();
+  if (G == 0) ml[(wave * BM + l16) * 2] = m, ml[(wave * BM + l16) * 2 + 1] = l;
+  if (l16 < rows) {
+    float* mine = reinterpret_cast<float*>(smem) + (wave * BM + l16) * PITCH + 4 * G;
+#pragma unroll
+    for (int c = 0; c < DC; ++c) *reinterpret_cast<f32x4*>(mine + 16 * c) = o[c];
+  }
+  __syncthreads();
+  constexpr int TPR = D / 4;
+  for (int idx = threadIdx.x; idx < rows * TPR; idx += 64 * NW) {
+    const int lr = idx / TPR, d0 = (idx % TPR) * 4;
+    float M = NONE, L = 0.f;
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < NW; ++k) M = fmaxf(M, ml[(k * BM + lr) * 2]);
+#pragma unroll
+    for (int k = 0; k < NW; ++k) {
+      const float w = __builtin_amdgcn_exp2f(ml[(k * BM + lr) * 2] - M);
+      L += ml[(k * BM + lr) * 2 + 1] * w;
+      const f32x4 y = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(smem) + (k * BM + lr) * PITCH + d0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] += y[e] * w;
+    }
+    if (part) {
+      const long slot = (long)blockIdx.x * BM + lr;
+      *reinterpret_cast<f32x4*>(a.ws + slot * D + d0) = f32x4{x[0], x[1], x[2], x[3]};
+      if (d0 == 0) *reinterpret_cast<f32x2*>(a.ws + a.ws_ml + slot * 2) = f32x2{M, L};
+    } else {
+      const int rr = row0 + lr, t = fdiv(rr, a.g);
+      store_row<T, 4>(a, it.q.q0 + t, it.head * (int)a.g.d + rr - t * (int)a.g.d, d0, x, M, L);
+    }
+  }
+}
+
 // Joins the chunks of a (tile, head): D / 4 threads a row.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a, int BM, int KU) {
+template <typename T, int D, int BM, int KU>
+__global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a) {
   Item it;
   const int lane = threadIdx.x & 63;
-  if (!find_item(a, blockIdx.x, lane, BM, KU, 1, it)) return;
+  if (!find_item<BM, KU, true>(a, blockIdx.x, lane, it)) return;
   if (it.nch <= 1) return;
   constexpr int TPR = D / 4;
   const int R = it.q.n * (int)a.g.d;
@@ -525,14 +865,15 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a, int 
   const int d0 = (threadIdx.x % TPR) * 4;
   const int end = min(tile_end(a, it, BM), (it.u0 + it.units) * KU);
   const int left = end - it.u0 * KU;
-  const int n = left > 0 ? (left + it.cs * KU - 1) / (it.cs * KU) : 1;  // chunks that wrote
+  const int n = left > 0 ? ((left + KU - 1) / KU + it.cs - 1) / it.cs : 1;  // chunks that wrote
   if (it.first + (long)(n - 1) * it.step >= a.items) return;  // only where q_start descends
   const float* ml = a.ws + a.ws_ml;
+  const long s0 = (long)it.first * BM + lr, ds = (long)it.step * BM;
   float M = NONE;
-  for (int c = 0; c < n; ++c) M = fmaxf(M, ml[((it.first + (long)c * it.step) * BM + lr) * 2]);
+  for (int c = 0; c < n; ++c) M = fmaxf(M, ml[(s0 + c * ds) * 2]);
   float x[4] = {0.f, 0.f, 0.f, 0.f}, L = 0.f;
   for (int c = 0; c < n; ++c) {
-    const long slot = (it.first + (long)c * it.step) * BM + lr;
+    const long slot = s0 + c * ds;
     const f32x2 p = *reinterpret_cast<const f32x2*>(ml + slot * 2);
     const f32x4 y = *reinterpret_cast<const f32x4*>(a.ws + slot * D + d0);
     const float w = __builtin_amdgcn_exp2f(p[0] - M);
@@ -564,18 +905,17 @@ int device_cus() {
   return cus[dev];
 }
 
-// Few rows for each sequence and key/value head: 32-row tiles whose four waves share out the keys.  Otherwise
-// 128-row tiles whose four waves share the keys.
-bool few_rows(long rows, int S, int g) { return rows * g <= 32l * S; }
-
+// At most 16 rows for each sequence and key/value head on average (single tokens of groups up to 16): the kernel for
+// few rows.  Otherwise 128-row tiles whose four waves share the keys.
 Plan make_plan(long rows, int S, int Hq, int Hk, int D, long most) {
   Plan p;
-  const int g = Hq / Hk;
-  const bool few = few_rows(rows, S, g);
-  p.BM = few ? 32 : 128;
-  p.KU = few ? (D > 128 ? 128 : 128) : 64;
-  p.pairs = (rows * g / p.BM + S) * Hk;
-  p.slots = device_cus() * 2;
+  const long g = Hq / Hk;
+  const bool few = rows * g <= 16l * S;
+  p.BM = few ? 16 : 128;
+  p.KU = few ? 128 : 64;
+  const long a = rows * g / p.BM + S, b = rows * ((g + p.BM - 1) / p.BM);
+  p.pairs = (a < b ? a : b) * Hk;
+  p.slots = device_cus() * (D <= 128 ? 2 : 1);
   const long least = (rows * g + p.BM - 1) / p.BM * Hk;
   p.split = most > p.KU && least < 8l * p.slots;
   p.items = p.split ? p.pairs + 4l * p.slots : p.pairs;
@@ -584,20 +924,28 @@ Plan make_plan(long rows, int S, int Hq, int Hk, int D, long most) {
   return p;
 }
 
+template <typename T, int D, int BM, int KU>
+int join(PagedArgs& a, const Plan& p, hipStream_t st) {
+  OSPO_CHECK_LAUNCH();
+  if (!p.split) return OSPO_OK;
+  constexpr int RPB = 256 / (D / 4);
+  paged_join_kernel<T, D, BM, KU><<<dim3((unsigned)p.pairs, (BM + RPB - 1) / RPB), 256, 0, st>>>(a);
+  OSPO_CHECK_LAUNCH();
+  return OSPO_OK;
+}
+
 template <typename T, int D>
 int launch(PagedArgs& a, const Plan& p, hipStream_t st) {
   const dim3 grid((unsigned)p.items);
-  if (p.BM == 32)
-    paged_attn_kernel<T, D, 1, 1, 4, 32><<<grid, 256, 0, st>>>(a);
-  else
-    paged_attn_kernel<T, D, 1, 4, 1, 64><<<grid, 256, 0, st>>>(a);
-  OSPO_CHECK_LAUNCH();
-  if (p.split) {
-    constexpr int RPB = 256 / (D / 4);
-    paged_join_kernel<T, D><<<dim3((unsigned)p.pairs, (unsigned)((p.BM + RPB - 1) / RPB)), 256, 0, st>>>(a, p.BM, p.KU);
-    OSPO_CHECK_LAUNCH();
+  if (p.BM == 16) {
+    if (a.ps.d % 16 == 0)
+      paged_few_kernel<T, D, true><<<grid, 256, 0, st>>>(a);
+    else
+      paged_few_kernel<T, D, false><<<grid, 256, 0, st>>>(a);
+    return join<T, D, 16, 128>(a, p, st);
   }
-  return OSPO_OK;
+  paged_attn_kernel<T, D, 1, 4, 1, 64><<<grid, 256, 0, st>>>(a);
+  return join<T, D, 128, 64>(a, p, st);
 }
 
 bool shapes_ok(int n, int S, int Hq, int Hk, int D, int n_pages, int page_size, int max_pages) {
