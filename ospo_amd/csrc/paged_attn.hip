@@ -13,6 +13,8 @@
 // (maximum, sum, O) in fp32 and a second launch joins them in chunk order: no atomics, the same bits each time.
 #include <math.h>
 
+#include <type_traits>
+
 #include "paged.h"
 
 namespace {
@@ -193,6 +195,7 @@ template <>
 struct Frag<bf16> {
   typedef bf16x8 v8;
   static constexpr unsigned EXP = 0x7f80, MAN = 0x007f;
+  static constexpr float GROW = 24.f;
   __device__ static f32x16 mma(const v8& x, const v8& y, const f32x16& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0);
   }
@@ -201,6 +204,7 @@ template <>
 struct Frag<f16> {
   typedef f16x8 v8;
   static constexpr unsigned EXP = 0x7c00, MAN = 0x03ff;
+  static constexpr float GROW = 12.f;
   __device__ static f32x16 mma(const v8& x, const v8& y, const f32x16& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0);
   }
@@ -239,6 +243,13 @@ __device__ __forceinline__ i16x4 read_tr(const char* src) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS i16x4*)src);
 }
 
+// barrier of the workgroup behind this wave's LDS accesses (loads and LDS-DMA from memory stay in flight)
+__device__ __forceinline__ void sync_lds() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 __device__ __forceinline__ float other_half(float x) {  // the value of lane ^ 32
   const unsigned u = __float_as_uint(x);
   const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
@@ -265,49 +276,51 @@ __device__ __forceinline__ void store_row(const PagedArgs& a, int tok, int hd, i
 
 constexpr int pitch_of(int D) { return D + 4; }  // floats of a staged output row
 
-template <int D, int WR, int WK, int KT>
-constexpr int lds_bytes() {
-  const int kv = WK * 2 * KT * D * 2;
-  const int out = WR * WK * 32 * pitch_of(D) * 4 + WR * WK * 32 * 8;
-  return kv > out ? kv : out;
-}
-
-// WR waves along the rows (32 RB each), WK along the keys; a wave's key tiles are KT keys wide.
-template <typename T, int D, int RB, int WR, int WK, int KT>
-__global__ __launch_bounds__(64 * WR * WK) void paged_attn_kernel(const PagedArgs a) {
+// ---------------------------------------------------------------- many rows
+// Chunks and prompts: the matrix unit bounds it.  Four waves of 32 RB rows share tiles of 64 keys; a wave's 64 rows
+// (RB = 2) feed two products from each fragment that it reads, so that LDS is read at half its rate (32 rows would
+// need all of it).  One wave a SIMD, so its own instruction stream has to keep the matrix unit fed, in steps of 32
+// keys: while step i's scores become probabilities (vector unit), step i + 1's scores are formed (matrix unit);
+// while O takes step i, the sums of step i and the maxima of step i + 1 are taken.  (Steps of 64 keys need more
+// vector registers than there are.)
+// K(j + 2) and V(j + 1) come by LDS-DMA with a whole tile's time to arrive.
+// The running maximum is raised (and O rescaled) only when some row's grew by more than GROW powers of two (24 in
+// bf16, 12 in fp16): probabilities then reach at most 2^GROW, which both types hold with no loss of relative
+// precision, and sums stay in fp32.
+template <typename T, int D, int RB, bool P16>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void paged_many_kernel(const PagedArgs a) {
   using F = Frag<T>;
   using v8 = typename F::v8;
-  constexpr int BM = 32 * RB * WR, KU = KT * WK, NT = 64 * WR * WK;
-  constexpr int ROWB = D * 2, CH = D / 8;
-  constexpr int KS = D / 16;  // d steps of S
-  constexpr int DC = D / 32;  // d chains of O
-  constexpr int KB = KT / 32;  // key blocks of S
-  __shared__ __attribute__((aligned(16))) char smem[lds_bytes<D, WR, WK, KT>()];
+  constexpr int NW = 4, BM = 32 * RB * NW, KU = 64;
+  constexpr int ROWB = D * 2, CH = D / 8, TILE = KU * ROWB;
+  constexpr int KS = D / 16, DC = D / 32;
+  constexpr int NL = D / 32, RPL = 64 / CH;  // 16-byte loads a lane for its wave's 16 rows of a tile; rows of one
+  // objects of their own, so that the compiler sees that a read of one does not wait for what is on its way to another
+  __shared__ __attribute__((aligned(1024))) char K0[TILE], K1[TILE], V0[TILE], V1[TILE];
+  __shared__ int inf[NW][RB * DC][64];  // where a sum is +infinity (bit r) and -infinity (bit 16 + r), see mend
+  __shared__ int found;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wr = wave % WR, wk = wave / WR;
   const int hi = lane >> 5, l32 = lane & 31;
 
   Item it;
   if (!find_item<BM, KU, false>(a, blockIdx.x, lane, it)) return;
-  const int R = it.q.n * (int)a.g.d;  // rows of the sequence
+  const int R = it.q.n * (int)a.g.d;
   const int ub = it.u0 + it.chunk * it.cs;
-  const int kb = ub * KU;  // the chunk's keys: kb (a multiple of KU) .. ke - 1
+  const int kb = ub * KU;
   const int ke = min(min(ub + it.cs, it.u0 + it.units) * KU, tile_end(a, it, BM));
   const bool part = it.nch > 1;
   if (part && it.chunk > 0 && kb >= ke) return;  // the joining launch counts the same chunks
-  const int row0 = it.tile * BM + wr * 32 * RB;
+  const int R0 = it.tile * BM, row0 = R0 + wave * 32 * RB;
 
   // rows of this lane: row0 + 32 b + l32 (rows behind the last repeat it and are not stored)
   v8 qf[RB][KS];
-  int lim[RB], low = 0x7fffffff, high = -1;
+  int lim[RB];
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
     const int r = min(row0 + 32 * b + l32, R - 1);
     const int tok = fdiv(r, a.g), hd = it.head * (int)a.g.d + r - tok * (int)a.g.d;
     lim[b] = a.causal ? it.q.kv - it.q.n + tok : it.q.kv - 1;
-    low = min(low, lim[b]);
-    high = max(high, lim[b]);
     const T* p = (const T*)a.q + (long)(it.q.q0 + tok) * a.q_ts + (long)hd * a.q_hs + 8 * hi;
     if (a.qvec) {
 #pragma unroll
@@ -319,214 +332,354 @@ __global__ __launch_bounds__(64 * WR * WK) void paged_attn_kernel(const PagedArg
         for (int i = 0; i < 8; ++i) qf[b][ks][i] = p[16 * ks + i];
     }
   }
-  // the wave's smallest and largest limit: tiles behind the latter are left out, tiles up to the former whole
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) {
-    low = min(low, __shfl_xor(low, s, 64));
-    high = max(high, __shfl_xor(high, s, 64));
-  }
-  low = __builtin_amdgcn_readfirstlane(low);
-  high = __builtin_amdgcn_readfirstlane(row0 < R ? high : -1);
+  // smallest limit of the wave's rows: tiles that end at or before it need no mask
+  const int low = a.causal ? it.q.kv - it.q.n + fdiv(min(row0, R - 1), a.g) : it.q.kv - 1;
 
-  f32x16 o[RB][DC];
-  float m[RB], l[RB];
+  f32x16 o[RB][DC], s[2][RB];
+  float m[RB], l[RB], mx[RB];
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
-    m[b] = NONE, l[b] = 0.f;
+    m[b] = NONE, l[b] = 0.f, mx[b] = -INFINITY;
 #pragma unroll
     for (int c = 0; c < DC; ++c)
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[b][c][r] = 0.f;
   }
+  const int n = ke > kb ? (ke - kb + KU - 1) / KU : 0;  // tiles
 
-  char* kl = smem + wk * 2 * KT * ROWB;  // this key group's K image, then V's
-  char* vl = kl + KT * ROWB;
+  // ---- memory to registers: this wave's 16 rows of a tile
   const T* kc = (const T*)a.kc + (long)it.head * a.c_hs;
   const T* vc = (const T*)a.vc + (long)it.head * a.c_hs;
   const int* bt = a.bt + (long)it.seq * a.max_pages;
-  const int steps = ke > kb ? (ke - kb + KU - 1) / KU : 0;
-  for (int t = 0; t < steps; ++t) {
-    const int k0 = kb + t * KU + wk * KT;  // this wave's tile
-    __syncthreads();
-    if (k0 < ke) {
-      constexpr int RPP = 1024 / ROWB;  // rows of a 1-KiB piece (one LDS-DMA of the wave)
+  const int lrow = lane / CH, lcol = (lane % CH) * 8;
+  const int lastp = ke > 0 ? fdiv(ke - 1, a.ps) : 0;
+  const int wrow = 16 * wave;
+  int scol[NL];  // column that this lane fetches for piece i: the chunk that the swizzle puts at its place
 #pragma unroll
-      for (int p = 0; p < KT / RPP / WR; ++p) {
-        const int piece = wr + WR * p;
-        const int row = piece * RPP + lane / CH;
-        const int key = min(k0 + row, ke - 1);
-        const int pi = fdiv(key, a.ps);
-        const int page = min(max(bt[pi], 0), a.n_pages - 1);
-        const long off = (long)page * a.c_ps + (long)(key - pi * (int)a.ps.d) * a.c_ts +
-                         (((lane % CH) ^ swz<D>(row)) << 3);
-        dma16(kc + off, kl + piece * 1024);
-        dma16(vc + off, vl + piece * 1024);
+  for (int i = 0; i < NL; ++i) scol[i] = ((lane % CH) ^ swz<D>(wrow + i * RPL + lrow)) * 8;
+  struct At {  // element offsets of the wave's rows of a tile
+    long u;  // P16: of the first (uniform)
+    long v[P16 ? 1 : NL];
+  };
+  int pbase = 0, pv = 0, pn = 0, pg[NL];
+  auto clampp = [&](int p) __attribute__((always_inline)) { return min(max(p, 0), a.n_pages - 1); };
+  auto lookup = [&](int k0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) pg[i] = bt[fdiv(min(k0 + wrow + i * RPL + lrow, ke - 1), a.ps)];
+  };
+  auto place = [&](int t, At& at) __attribute__((always_inline)) {
+    const int k0 = kb + t * KU;
+    if constexpr (P16) {
+      const int pi = fdiv(k0 + wrow, a.ps), pc = min(pi, lastp);
+      if (pc - pbase >= 64) {
+        pbase += 64;
+        pv = clampp(pn);
+        pn = bt[min(pbase + 64 + lane, lastp)];
+      }
+      at.u = (long)lane_of(pv, pc - pbase) * a.c_ps + (long)(k0 + wrow - pi * (int)a.ps.d) * a.c_ts;
+    } else {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int key = min(k0 + wrow + i * RPL + lrow, ke - 1);
+        at.v[i] = (long)clampp(pg[i]) * a.c_ps + (long)(key - fdiv(key, a.ps) * (int)a.ps.d) * a.c_ts;
+      }
+      if (t + 1 < n) lookup(k0 + KU);
+    }
+  };
+  const int loff = lrow * (int)a.c_ts;
+  auto fetch = [&](const T* base, const At& at, char* buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      char* dst = buf + (wrow + i * RPL) * ROWB;
+      if constexpr (P16)
+        dma16(base + at.u + (long)(i * RPL) * a.c_ts + (loff + scol[i]), dst);
+      else
+        dma16(base + at.v[i] + scol[i], dst);
+    }
+  };
+
+  // ---- the parts of a step (t: tile, h: its 32-key half)
+  auto scores = [&](const char* kl, int h, f32x16 (&x)[RB]) __attribute__((always_inline)) {
+    const int row = 32 * h + l32;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const v8 kf = *reinterpret_cast<const v8*>(kl + row * ROWB + (((2 * ks + hi) ^ swz<D>(row)) << 4));
+#pragma unroll
+      for (int b = 0; b < RB; ++b) {
+        if (ks == 0) {
+          f32x16 z;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) z[r] = 0.f;
+          x[b] = F::mma(kf, qf[b][ks], z);
+        } else {
+          x[b] = F::mma(kf, qf[b][ks], x[b]);
+        }
       }
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (k0 >= ke || k0 > high) continue;
-    const bool mask = k0 < it.q.st || k0 + KT - 1 > low;
+  };
+  auto masked = [&](int t, int h) __attribute__((always_inline)) {
+    const int k0 = kb + t * KU + 32 * h;
+    return k0 < it.q.st || k0 + 31 > low;
+  };
+  auto hidden = [&](int b, int key) __attribute__((always_inline)) { return key > lim[b] || key < it.q.st; };
+  auto apply_mask = [&](int t, int h, f32x16 (&x)[RB]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        x[b][r] = hidden(b, kb + t * KU + 32 * h + (r & 3) + 8 * (r >> 2) + 4 * hi) ? -INFINITY : x[b][r];
+  };
+  auto maxima = [&](const f32x16 (&x)[RB]) __attribute__((always_inline)) {
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
-      f32x16 s[KB];
+      float y = x[b][0];
 #pragma unroll
-      for (int kk = 0; kk < KB; ++kk) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[kk][r] = 0.f;
-        const int row = 32 * kk + l32;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const v8 kf = *reinterpret_cast<const v8*>(kl + row * ROWB + (((2 * ks + hi) ^ swz<D>(row)) << 4));
-          s[kk] = F::mma(kf, qf[b][ks], s[kk]);
-        }
-      }
-      if (mask) {
-#pragma unroll
-        for (int kk = 0; kk < KB; ++kk)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int key = k0 + 32 * kk + (r & 3) + 8 * (r >> 2) + 4 * hi;
-            s[kk][r] = key > lim[b] || key < it.q.st ? -INFINITY : s[kk][r];
-          }
-      }
-      float mx = s[0][0];
-#pragma unroll
-      for (int kk = 0; kk < KB; ++kk)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kk][r]);
-      mx = fmaxf(mx, other_half(mx));
-      const float mn = fmaxf(m[b], mx * a.cs);
-      const float alpha = __builtin_amdgcn_exp2f(m[b] - mn);
-      m[b] = mn;
-      float sum = 0.f;
-#pragma unroll
-      for (int kk = 0; kk < KB; ++kk)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[kk][r] = __builtin_amdgcn_exp2f(fmaf(s[kk][r], a.cs, -mn));
-          sum += s[kk][r];
-        }
-      l[b] = l[b] * alpha + sum + other_half(sum);
-      // P in the cache's type (rounded to nearest: the matrix unit's operand; the sum above keeps fp32)
-      v8 pt[KT / 16];
-#pragma unroll
-      for (int u = 0; u < KT / 16; ++u)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) pt[u][i] = (T)s[u >> 1][8 * (u & 1) + i];
-      auto vfrag = [&](int c, int u) __attribute__((always_inline)) {
-        const int G = lane >> 4, li = lane & 15;
-        const int r1 = 16 * u + 4 * hi + (li >> 2), r2 = r1 + 8;
-        const int ch = 4 * c + 2 * (G & 1) + ((li & 3) >> 1), h8 = (li & 1) << 3;
-        const i16x4 x = read_tr(vl + r1 * ROWB + ((ch ^ swz<D>(r1)) << 4) + h8);
-        const i16x4 y = read_tr(vl + r2 * ROWB + ((ch ^ swz<D>(r2)) << 4) + h8);
-        return i16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-      };
-      if (!mask) {
-#pragma unroll
-        for (int c = 0; c < DC; ++c) {
-          o[b][c] *= alpha;
-#pragma unroll
-          for (int u = 0; u < KT / 16; ++u) o[b][c] = F::mma(__builtin_bit_cast(v8, vfrag(c, u)), pt[u], o[b][c]);
-        }
-      } else {
-        // A masked key has p = 0, but 0 times an infinity or NaN in its value would reach the row all the same.
-        // The tile's product is formed apart; where it is not finite, it is formed again with those values as
-        // zeros, and what rows that see them get is added: +inf, -inf or NaN, found by a product with the mask.
-#pragma unroll
-        for (int c = 0; c < DC; ++c) {
-          f32x16 x;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) x[r] = 0.f;
-#pragma unroll
-          for (int u = 0; u < KT / 16; ++u) x = F::mma(__builtin_bit_cast(v8, vfrag(c, u)), pt[u], x);
-          float bad = 0.f;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) bad = fmaf(x[r], 0.f, bad);
-          if (__ballot(bad != 0.f)) {
-            f32x16 up, dn;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) x[r] = up[r] = dn[r] = 0.f;
-            for (int u = 0; u < KT / 16; ++u) {
-              const i16x8 v = vfrag(c, u);
-              v8 fin, isup, isdn, seen;
-              const v8 pu = u == 0 ? pt[0] : u == 1 ? pt[1] : KT > 32 && u == 2 ? pt[KT > 32 ? 2 : 0] : pt[KT > 32 ? 3 : 1];
-split_values<T>(v, fin, isup, isdn);
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const int key = k0 + 16 * u + 4 * hi + (i & 3) + 8 * (i >> 2);
-                seen[i] = key > lim[b] || key < it.q.st ? (T)0.f : (T)1.f;
-              }
-              x = F::mma(fin, pu, x);
-              up = F::mma(isup, seen, up);
-              dn = F::mma(isdn, seen, dn);
-            }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              if (up[r] > 0.f) x[r] += INFINITY;
-              if (dn[r] > 0.f) x[r] -= INFINITY;
-            }
-          }
-          o[b][c] = o[b][c] * alpha + x;
-        }
-      }
+      for (int r = 1; r < 16; ++r) y = fmaxf(y, x[b][r]);
+      mx[b] = y;
     }
+  };
+  auto vfrag = [&](const char* vl, int c, int u) __attribute__((always_inline)) {
+    const int G = lane >> 4, li = lane & 15;
+    const int r1 = 16 * u + 4 * hi + (li >> 2), r2 = r1 + 8;
+    const int ch = 4 * c + 2 * (G & 1) + ((li & 3) >> 1), h8 = (li & 1) << 3;
+    const i16x4 x = read_tr(vl + r1 * ROWB + ((ch ^ swz<D>(r1)) << 4) + h8);
+    const i16x4 y = read_tr(vl + r2 * ROWB + ((ch ^ swz<D>(r2)) << 4) + h8);
+    return i16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+  };
+
+  // tiles that some row of the workgroup sees in part; whether one holds values that are not finite (flags, by V buffer)
+  const int low0 = a.causal ? it.q.kv - it.q.n + fdiv(R0, a.g) : it.q.kv - 1;
+  auto edge = [&](int t) __attribute__((always_inline)) { return kb + t * KU < it.q.st || kb + t * KU + KU - 1 > low0; };
+  auto look = [&](const char* vl) __attribute__((always_inline)) {
+    if (threadIdx.x == 0) found = 0;
+    sync_lds();
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(vl + (wrow + i * RPL) * ROWB + lane * 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) odd = odd || (x[e] & F::EXP) == F::EXP || (x[e] >> 16 & F::EXP) == F::EXP;
+    }
+    if (odd) found = 1;
+    sync_lds();
+    return found != 0;
+  };
+
+  At ak{}, av{};  // of K(j + 1) / V(j + 1) at the start of step j
+  if (n > 0) {
+    if constexpr (P16) {
+      pbase = fdiv(kb + wrow, a.ps);
+      if (pbase > lastp) pbase = lastp;
+      pv = clampp(bt[min(pbase + lane, lastp)]);
+      pn = bt[min(pbase + 64 + lane, lastp)];
+    } else {
+      lookup(kb);
+    }
+    At a0{};
+    place(0, a0);
+    fetch(kc, a0, K0);
+    fetch(vc, a0, V0);
+    if (n > 1) {
+      place(1, ak);
+      fetch(kc, ak, K1);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    sync_lds();
+    scores(K0, 0, s[0]);
+    if (masked(0, 0)) apply_mask(0, 0, s[0]);
+    maxima(s[0]);
+#pragma unroll
+    for (int b = 0; b < RB; ++b) m[b] = fmaxf(NONE, fmaxf(mx[b], other_half(mx[b])) * a.cs);
   }
 
-  // Join the key groups and store: rows through LDS, 16 bytes a lane.
-  const int R0 = it.tile * BM;
-  constexpr int PITCH = pitch_of(D);
-  float* ml = reinterpret_cast<float*>(smem + WR * WK * 32 * PITCH * 4);  // [wave][row] (m, l)
+  // A masked key has p = 0, but 0 times an infinity or NaN in its value would reach the row all the same.  Where a tile
+  // that some row sees in part holds such values (rare), they become zeros in LDS; which sums rows that see them
+  // get +infinity or -infinity into (NaN: both) is found by a product with the mask and kept until the end.
+  bool anyinf = false;
+  auto mend = [&](int j, char* vl) __attribute__((always_inline)) {
+    if (!anyinf)
+      for (int i = 0; i < RB * DC; ++i) inf[wave][i][lane] = 0;
+    anyinf = true;
+#pragma nounroll
+    for (int c = 0; c < DC; ++c)
 #pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    __syncthreads();
-    if (hi == 0) ml[(wave * 32 + l32) * 2] = m[b], ml[(wave * 32 + l32) * 2 + 1] = l[b];
-    __syncthreads();
-    float M = m[b];
+      for (int b = 0; b < RB; ++b) {
+        f32x16 up, dn;
 #pragma unroll
-    for (int k = 0; k < WK; ++k) M = fmaxf(M, ml[((k * WR + wr) * 32 + l32) * 2]);
-    const float w = __builtin_amdgcn_exp2f(m[b] - M);
-    float* mine = reinterpret_cast<float*>(smem) + (wave * 32 + l32) * PITCH;
+        for (int r = 0; r < 16; ++r) up[r] = dn[r] = 0.f;
+#pragma nounroll
+        for (int u = 0; u < 4; ++u) {
+          v8 fin, isup, isdn, seen;
+          split_values<T>(vfrag(vl, c, u), fin, isup, isdn);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            seen[i] = hidden(b, kb + j * KU + 16 * u + 4 * hi + (i & 3) + 8 * (i >> 2)) ? (T)0.f : (T)1.f;
+          up = F::mma(isup, seen, up);
+          dn = F::mma(isdn, seen, dn);
+        }
+        int bits = 0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) bits |= (up[r] > 0.f ? 1 << r : 0) | (dn[r] > 0.f ? 65536 << r : 0);
+        inf[wave][c * RB + b][lane] |= bits;
+      }
+    sync_lds();
+#pragma nounroll
+    for (int i = 0; i < NL; ++i) {
+      i16x8* x = reinterpret_cast<i16x8*>(vl + (wrow + i * RPL) * ROWB + lane * 16);
+      v8 fin, isup, isdn;
+      split_values<T>(*x, fin, isup, isdn);
+      *x = __builtin_bit_cast(i16x8, fin);
+    }
+    sync_lds();
+  };
+  // O taken out of the way when a maximum grew too much: acc = acc * alpha + O * alpha, O = 0.  In memory, and rare:
+  // vector registers have no room for O, and the matrix unit's own can only be added to.
+  volatile float acc[RB * DC * 16], out[RB * DC * 16];
+  bool flushed = false;
+  auto flush = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+      for (int c = 0; c < DC; ++c)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) out[(b * DC + c) * 16 + r] = o[b][c][r];
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      const float mn = fmaxf(m[b], mx[b]);
+      const float alpha = __builtin_amdgcn_exp2f(m[b] - mn);
+      m[b] = mn;
+      l[b] *= alpha;
+      for (int i = 0; i < DC * 16; ++i) {
+        const int e = b * DC * 16 + i;
+        const float old = flushed ? acc[e] : 0.f;
+        acc[e] = (old + out[e]) * alpha;
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+      for (int c = 0; c < DC; ++c)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[b][c][r] = 0.f;
+    flushed = true;
+  };
+  // half h of tile j: x its scores, y those of the next half (nk: its K image; more: there is one)
+  auto half = [&](int j, auto hc, const char* nk, const char* vl, bool more, f32x16 (&x)[RB], f32x16 (&y)[RB])
+                  __attribute__((always_inline)) {
+    constexpr int H = decltype(hc)::value;
+    // raise the maxima where they grew too much
+    bool grow = false;
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      mx[b] = fmaxf(mx[b], other_half(mx[b])) * a.cs;
+      grow = grow || mx[b] > m[b] + F::GROW;
+    }
+    if (__ballot(grow)) flush();
+    __builtin_amdgcn_sched_barrier(0);
+    // the next half's scores beside this half's exponentials
+    scores(nk, H ^ 1, y);  // (behind the last half: of what is there, and not used)
+    v8 pt[RB][2];
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(x[b][r], a.cs, -m[b]));
+        x[b][r] = p;
+        pt[b][r >> 3][r & 7] = (T)p;  // (rounded to nearest: the matrix unit's operand; the sums keep fp32)
+      }
+    // (here, not where they are used: the exponentials belong beside the scores' products)
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) asm volatile("" : "+v"(pt[b][u]));
+    __builtin_amdgcn_sched_barrier(0);
+    if (more && masked(j + H, H ^ 1)) apply_mask(j + H, H ^ 1, y);
 #pragma unroll
     for (int c = 0; c < DC; ++c)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        f32x4 x;
+      for (int u = 0; u < 2; ++u) {
+        const v8 v = __builtin_bit_cast(v8, vfrag(vl, c, 2 * H + u));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = o[b][c][4 * k + i] * w;
-        *reinterpret_cast<f32x4*>(mine + 32 * c + 8 * k + 4 * hi) = x;
+        for (int b = 0; b < RB; ++b) o[b][c] = F::mma(v, pt[b][u], o[b][c]);
       }
-    __syncthreads();
-    constexpr int TPR = D / 8;
-    for (int idx = threadIdx.x; idx < WR * 32 * TPR; idx += NT) {
-      const int lr = idx / TPR, d0 = (idx % TPR) * 8;
-      const int w_ = lr / 32, r32 = lr % 32;
-      const int r = R0 + w_ * 32 * RB + 32 * b + r32;
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) l[b] += x[b][r];
+    maxima(y);
+  };
+  auto step = [&](int j, char* k0, char* k1, char* v0, char* v1) __attribute__((always_inline)) {
+    // V(j + 1) lies where K(j + 1) did, and takes the place of V(j - 1)
+    av = ak;
+    if (j + 1 < n) fetch(vc, av, v1);
+    if (j + 2 < n) place(j + 2, ak);
+    if (edge(j) && look(v0)) mend(j, v0);
+    half(j, std::integral_constant<int, 0>{}, k0, v0, true, s[0], s[1]);
+    // K(j + 1) is there (behind it: only V(j + 1) and page numbers), and every wave has read K(j)
+    if (j + 1 < n) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
+    sync_lds();
+    if (j + 2 < n) fetch(kc, ak, k0);
+    half(j, std::integral_constant<int, 1>{}, k1, v0, j + 1 < n, s[1], s[0]);
+    // V(j + 1) is there
+    if (j + 2 < n)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    sync_lds();
+  };
+  for (int j = 0; j < n; j += 2) {
+    step(j, K0, K1, V0, V1);
+    if (j + 1 < n) step(j + 1, K1, K0, V1, V0);
+  }
+
+  // Rows through LDS (the tiles' room: 32 rows of D floats a wave, their 16-byte chunks turned by the row), stored 16
+  // bytes a lane.
+  float* st = reinterpret_cast<float*>(wave == 0 ? K0 : wave == 1 ? K1 : wave == 2 ? V0 : V1);
+  auto at = [&](int row, int chunk) __attribute__((always_inline)) { return row * D + ((chunk ^ (row & (D / 4 - 1) & 31)) << 2); };
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    const float L = l[b] + other_half(l[b]);
+#pragma unroll
+    for (int c = 0; c < DC; ++c)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        *reinterpret_cast<f32x4*>(st + at(l32, 8 * c + 2 * k + hi)) =
+            f32x4{o[b][c][4 * k], o[b][c][4 * k + 1], o[b][c][4 * k + 2], o[b][c][4 * k + 3]};
+    if (flushed || anyinf)
+      for (int i = 0; i < DC * 16; ++i) {
+        float* e = st + at(l32, 8 * (i >> 4) + 2 * (i >> 2 & 3) + hi) + (i & 3);
+        float x = *e;
+        if (flushed) x += acc[b * DC * 16 + i];
+        if (anyinf) {
+          const int bits = inf[wave][(i >> 4) * RB + b][lane] >> (i & 15);
+          if (bits & 1) x += INFINITY;
+          if (bits & 65536) x -= INFINITY;
+        }
+        *e = x;
+      }
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32 / RPL; ++i) {
+      const int lr = i * RPL + lrow, r = row0 + 32 * b + lr;
+      const float Lr = __shfl(L, lr, 64), Mr = __shfl(m[b], lr, 64);
+      const f32x4 x0 = *reinterpret_cast<const f32x4*>(st + at(lr, lcol / 4));
+      const f32x4 x1 = *reinterpret_cast<const f32x4*>(st + at(lr, lcol / 4 + 1));
       if (r >= R) continue;
-      float x[8], M2 = NONE, L = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = 0.f;
-#pragma unroll
-      for (int k = 0; k < WK; ++k) M2 = fmaxf(M2, ml[((k * WR + w_) * 32 + r32) * 2]);
-#pragma unroll
-      for (int k = 0; k < WK; ++k) {
-        const int wv = k * WR + w_;
-        L += ml[(wv * 32 + r32) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(wv * 32 + r32) * 2] - M2);
-        const float* y = reinterpret_cast<const float*>(smem) + (wv * 32 + r32) * PITCH + d0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] += y[i];
-      }
-      const int tok = fdiv(r, a.g), hd = it.head * (int)a.g.d + r - tok * (int)a.g.d;
       if (part) {
         const long slot = (long)blockIdx.x * BM + (r - R0);
-        float* y = a.ws + slot * D + d0;
-        *reinterpret_cast<f32x4*>(y) = f32x4{x[0], x[1], x[2], x[3]};
-        *reinterpret_cast<f32x4*>(y + 4) = f32x4{x[4], x[5], x[6], x[7]};
-        if (d0 == 0) *reinterpret_cast<f32x2*>(a.ws + a.ws_ml + slot * 2) = f32x2{M2, L};
+        *reinterpret_cast<f32x4*>(a.ws + slot * D + lcol) = x0;
+        *reinterpret_cast<f32x4*>(a.ws + slot * D + lcol + 4) = x1;
+        if (lcol == 0) *reinterpret_cast<f32x2*>(a.ws + a.ws_ml + slot * 2) = f32x2{Mr, Lr};
       } else {
-        store_row<T, 8>(a, it.q.q0 + tok, hd, d0, x, M2, L);
+        const int tok = fdiv(r, a.g), hd = it.head * (int)a.g.d + r - tok * (int)a.g.d;
+        const float x[8] = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
+        store_row<T, 8>(a, it.q.q0 + tok, hd, lcol, x, Mr, Lr);
       }
     }
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
 }
 
@@ -769,7 +922,7 @@ __global__ __launch_bounds__(256) void paged_few_kernel(const PagedArgs a) {
         if (!mask) {
           o[c4 + c] = Mma16<T>::mma(__builtin_bit_cast(v8, vv), pt, o[c4 + c] * alpha);
         } else {
-          // a value that some row doesn't see must not reach it, whatever it is: see paged_attn_kernel
+          // a value that some row doesn't see must not reach it, whatever it is: see paged_many_kernel
           f32x4 x = Mma16<T>::mma(__builtin_bit_cast(v8, vv), pt, f32x4{0.f, 0.f, 0.f, 0.f});
           float bad = 0.f;
 #pragma unroll
@@ -906,16 +1059,17 @@ int device_cus() {
 }
 
 // At most 16 rows for each sequence and key/value head on average (single tokens of groups up to 16): the kernel for
-// few rows.  Otherwise 128-row tiles whose four waves share the keys.
+// few rows.  Otherwise the one for many (256-row tiles; 128 with 256-wide heads, whose O fills the registers at 32 rows
+// a wave).
 Plan make_plan(long rows, int S, int Hq, int Hk, int D, long most) {
   Plan p;
   const long g = Hq / Hk;
   const bool few = rows * g <= 16l * S;
-  p.BM = few ? 16 : 128;
+  p.BM = few ? 16 : D > 128 ? 128 : 256;
   p.KU = few ? 128 : 64;
   const long a = rows * g / p.BM + S, b = rows * ((g + p.BM - 1) / p.BM);
   p.pairs = (a < b ? a : b) * Hk;
-  p.slots = device_cus() * (D <= 128 ? 2 : 1);
+  p.slots = device_cus() * (few && D <= 128 ? 2 : 1);
   const long least = (rows * g + p.BM - 1) / p.BM * Hk;
   p.split = most > p.KU && least < 8l * p.slots;
   p.items = p.split ? p.pairs + 4l * p.slots : p.pairs;
@@ -944,8 +1098,12 @@ int launch(PagedArgs& a, const Plan& p, hipStream_t st) {
       paged_few_kernel<T, D, false><<<grid, 256, 0, st>>>(a);
     return join<T, D, 16, 128>(a, p, st);
   }
-  paged_attn_kernel<T, D, 1, 4, 1, 64><<<grid, 256, 0, st>>>(a);
-  return join<T, D, 128, 64>(a, p, st);
+  constexpr int RB = D > 128 ? 1 : 2;
+  if (a.ps.d % 16 == 0)
+    paged_many_kernel<T, D, RB, true><<<grid, 256, 0, st>>>(a);
+  else
+    paged_many_kernel<T, D, RB, false><<<grid, 256, 0, st>>>(a);
+  return join<T, D, 128 * RB, 64>(a, p, st);
 }
 
 bool shapes_ok(int n, int S, int Hq, int Hk, int D, int n_pages, int page_size, int max_pages) {
