@@ -189,6 +189,11 @@ __device__ __forceinline__ int tile_end(const PagedArgs& a, const Item& it, int 
 }
 
 // ---------------------------------------------------------------- types
+// mma: a product as the compiler sees it.  acc: one into accumulators that stay in the matrix unit's own registers (the
+// compiler moves some of O to vector registers and back around its products).  It knows nothing of the waits that
+// such a product needs: two states behind the vector unit's last write to an operand, which the block brings along,
+// and settle() before anything but another product reads the accumulators.
+__device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 7" ::: "memory"); }
 template <typename T>
 struct Frag;
 template <>
@@ -196,6 +201,12 @@ struct Frag<bf16> {
   typedef bf16x8 v8;
   static constexpr unsigned EXP = 0x7f80, MAN = 0x007f;
   static constexpr float GROW = 24.f;
+  __device__ static void acc(f32x16& c, const bf16x8& x, const bf16x8& y) {
+    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(x), "v"(y));
+  }
+  __device__ static void clear(f32x16& c, const bf16x8& zero) {
+    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %1, 0" : "=a"(c) : "v"(zero));
+  }
   __device__ static f32x16 mma(const v8& x, const v8& y, const f32x16& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0);
   }
@@ -205,6 +216,12 @@ struct Frag<f16> {
   typedef f16x8 v8;
   static constexpr unsigned EXP = 0x7c00, MAN = 0x03ff;
   static constexpr float GROW = 12.f;
+  __device__ static void acc(f32x16& c, const f16x8& x, const f16x8& y) {
+    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(c) : "v"(x), "v"(y));
+  }
+  __device__ static void clear(f32x16& c, const f16x8& zero) {
+    asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %1, 0" : "=a"(c) : "v"(zero));
+  }
   __device__ static f32x16 mma(const v8& x, const v8& y, const f32x16& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0);
   }
@@ -280,13 +297,17 @@ constexpr int pitch_of(int D) { return D + 4; }  // floats of a staged output ro
 // Chunks and prompts: the matrix unit bounds it.  Four waves of 32 RB rows share tiles of 64 keys; a wave's 64 rows
 // (RB = 2) feed two products from each fragment that it reads, so that LDS is read at half its rate (32 rows would
 // need all of it).  One wave a SIMD, so its own instruction stream has to keep the matrix unit fed, in steps of 32
-// keys: while step i's scores become probabilities (vector unit), step i + 1's scores are formed (matrix unit);
-// while O takes step i, the sums of step i and the maxima of step i + 1 are taken.  (Steps of 64 keys need more
-// vector registers than there are.)
-// K(j + 2) and V(j + 1) come by LDS-DMA with a whole tile's time to arrive.
-// The running maximum is raised (and O rescaled) only when some row's grew by more than GROW powers of two (24 in
+// keys: while scores of tile j become probabilities (vector unit), those of tile j + 1 are formed (matrix unit);
+// while O takes tile j, sums of tile j and maxima of tile j + 1 are taken.  (64 keys at a time need more vector
+// registers than there are.)  K(j + 2) and V(j + 1) come by LDS-DMA with the whole tile's time to arrive: one barrier
+// a tile.
+// The running maximum is raised (and O put aside) only when some row's grew by more than GROW powers of two (24 in
 // bf16, 12 in fp16): probabilities then reach at most 2^GROW, which both types hold with no loss of relative
 // precision, and sums stay in fp32.
+//
+// LDS images: blocks of 16 keys x 32 columns, 1 KiB each, [16-byte chunk q of the columns][key, for V key ^ 4 q]: every
+// fragment is one address and a constant, and the reads of K (16 keys of a chunk) and the transposed reads of V (4
+// keys x 4 chunks by half a wave) meet every bank once.
 template <typename T, int D, int RB, bool P16>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void paged_many_kernel(const PagedArgs a) {
   using F = Frag<T>;
@@ -294,7 +315,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   constexpr int NW = 4, BM = 32 * RB * NW, KU = 64;
   constexpr int ROWB = D * 2, CH = D / 8, TILE = KU * ROWB;
   constexpr int KS = D / 16, DC = D / 32;
-  constexpr int NL = D / 32, RPL = 64 / CH;  // 16-byte loads a lane for its wave's 16 rows of a tile; rows of one
+  constexpr int NL = D / 32;    // column blocks: LDS-DMA pieces of a wave's 16 keys
+  constexpr int RPL = 64 / CH;  // rows of a 1-KiB store
   // objects of their own, so that the compiler sees that a read of one does not wait for what is on its way to another
   __shared__ __attribute__((aligned(1024))) char K0[TILE], K1[TILE], V0[TILE], V1[TILE];
   __shared__ int inf[NW][RB * DC][64];  // where a sum is +infinity (bit r) and -infinity (bit 16 + r), see mend
@@ -335,43 +357,53 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   // smallest limit of the wave's rows: tiles that end at or before it need no mask
   const int low = a.causal ? it.q.kv - it.q.n + fdiv(min(row0, R - 1), a.g) : it.q.kv - 1;
 
-  f32x16 o[RB][DC], s[2][RB];
-  float m[RB], l[RB], mx[RB];
+  f32x16 o[RB][DC], s[2][2][RB];  // scores: [tile parity][half]
+  float m[RB], l[RB], mx[2][RB];
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
-    m[b] = NONE, l[b] = 0.f, mx[b] = -INFINITY;
-#pragma unroll
-    for (int c = 0; c < DC; ++c)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[b][c][r] = 0.f;
+    m[b] = NONE, l[b] = 0.f, mx[0][b] = mx[1][b] = -INFINITY;
   }
+  auto settle = [&]() __attribute__((always_inline)) {  // (a product takes 16 passes at most: 18 states)
+    asm volatile("s_nop 15\n\ts_nop 7" ::: "memory");
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+      for (int c = 0; c < DC; ++c) asm volatile("" : "+a"(o[b][c]));
+  };
+  auto clear_o = [&]() __attribute__((always_inline)) {
+    v8 zero;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) zero[i] = (T)0.f;
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+      for (int c = 0; c < DC; ++c) F::clear(o[b][c], zero);
+  };
+  clear_o();
   const int n = ke > kb ? (ke - kb + KU - 1) / KU : 0;  // tiles
 
-  // ---- memory to registers: this wave's 16 rows of a tile
+  // ---- memory to LDS: this wave's 16 keys of a tile
   const T* kc = (const T*)a.kc + (long)it.head * a.c_hs;
   const T* vc = (const T*)a.vc + (long)it.head * a.c_hs;
   const int* bt = a.bt + (long)it.seq * a.max_pages;
-  const int lrow = lane / CH, lcol = (lane % CH) * 8;
   const int lastp = ke > 0 ? fdiv(ke - 1, a.ps) : 0;
-  const int wrow = 16 * wave;
-  int scol[NL];  // column that this lane fetches for piece i: the chunk that the swizzle puts at its place
-#pragma unroll
-  for (int i = 0; i < NL; ++i) scol[i] = ((lane % CH) ^ swz<D>(wrow + i * RPL + lrow)) * 8;
-  struct At {  // element offsets of the wave's rows of a tile
-    long u;  // P16: of the first (uniform)
-    long v[P16 ? 1 : NL];
+  const int wrow = 16 * wave, q4 = lane >> 4;
+  const int lkey[2] = {lane & 15, (lane & 15) ^ (q4 << 2)};  // key of this lane in a piece of K, of V
+  struct At {  // element offsets: of the wave's first key (uniform; 16 keys lie in one page), or of this lane's two keys
+    long u;
+    long v[2];
   };
-  int pbase = 0, pv = 0, pn = 0, pg[NL];
+  int pbase = 0, pv = 0, pn = 0, pg[2];
   auto clampp = [&](int p) __attribute__((always_inline)) { return min(max(p, 0), a.n_pages - 1); };
   auto lookup = [&](int k0) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < NL; ++i) pg[i] = bt[fdiv(min(k0 + wrow + i * RPL + lrow, ke - 1), a.ps)];
+    for (int i = 0; i < 2; ++i) pg[i] = bt[fdiv(min(k0 + wrow + lkey[i], ke - 1), a.ps)];
   };
   auto place = [&](int t, At& at) __attribute__((always_inline)) {
     const int k0 = kb + t * KU;
     if constexpr (P16) {
       const int pi = fdiv(k0 + wrow, a.ps), pc = min(pi, lastp);
-      if (pc - pbase >= 64) {
+      if (pc - pbase >= 64) {  // 64 page numbers sit on the lanes, the next 64 are on their way
         pbase += 64;
         pv = clampp(pn);
         pn = bt[min(pbase + 64 + lane, lastp)];
@@ -379,31 +411,38 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       at.u = (long)lane_of(pv, pc - pbase) * a.c_ps + (long)(k0 + wrow - pi * (int)a.ps.d) * a.c_ts;
     } else {
 #pragma unroll
-      for (int i = 0; i < NL; ++i) {
-        const int key = min(k0 + wrow + i * RPL + lrow, ke - 1);
-        at.v[i] = (long)clampp(pg[i]) * a.c_ps + (long)(key - fdiv(key, a.ps) * (int)a.ps.d) * a.c_ts;
+      for (int i = 0; i < 2; ++i) {
+        const int key = min(k0 + wrow + lkey[i], ke - 1);
+        at.v[i] = (long)clampp(pg[i]) * a.c_ps + (long)(key - fdiv(key, a.ps) * (int)a.ps.d) * a.c_ts + 8 * q4;
       }
       if (t + 1 < n) lookup(k0 + KU);
     }
   };
-  const int loff = lrow * (int)a.c_ts;
-  auto fetch = [&](const T* base, const At& at, char* buf) __attribute__((always_inline)) {
+  const int loff[2] = {lkey[0] * (int)a.c_ts + 8 * q4, lkey[1] * (int)a.c_ts + 8 * q4};
+  auto fetch = [&](const T* base, const At& at, int i, char* buf) __attribute__((always_inline)) {
+    const T* src = P16 ? base + at.u + loff[i] : base + at.v[i];
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      char* dst = buf + (wrow + i * RPL) * ROWB;
-      if constexpr (P16)
-        dma16(base + at.u + (long)(i * RPL) * a.c_ts + (loff + scol[i]), dst);
-      else
-        dma16(base + at.v[i] + scol[i], dst);
-    }
+    for (int p = 0; p < NL; ++p) dma16(src + 32 * p, buf + (4 * p + wave) * 1024);
+  };
+
+  // ---- fragments
+  const int kat = (l32 >> 4) * 1024 + hi * 256 + (l32 & 15) * 16;
+  auto kfrag = [&](const char* kl, int h, int ks) __attribute__((always_inline)) {
+    return *reinterpret_cast<const v8*>(kl + kat + (ks >> 1) * 4096 + (ks & 1) * 512 + h * 2048);
+  };
+  const int vq = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), vr = 4 * hi + ((lane & 15) >> 2);
+  const int vat0 = vq * 256 + (vr ^ (vq << 2)) * 16 + (lane & 1) * 8;
+  const int vat1 = vq * 256 + ((vr + 8) ^ (vq << 2)) * 16 + (lane & 1) * 8;
+  auto vfrag = [&](const char* vl, int c, int u) __attribute__((always_inline)) {
+    const i16x4 x = read_tr(vl + vat0 + (4 * c + u) * 1024), y = read_tr(vl + vat1 + (4 * c + u) * 1024);
+    return i16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
   };
 
   // ---- the parts of a step (t: tile, h: its 32-key half)
   auto scores = [&](const char* kl, int h, f32x16 (&x)[RB]) __attribute__((always_inline)) {
-    const int row = 32 * h + l32;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      const v8 kf = *reinterpret_cast<const v8*>(kl + row * ROWB + (((2 * ks + hi) ^ swz<D>(row)) << 4));
+      const v8 kf = kfrag(kl, h, ks);
 #pragma unroll
       for (int b = 0; b < RB; ++b) {
         if (ks == 0) {
@@ -417,126 +456,85 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       }
     }
   };
-  auto masked = [&](int t, int h) __attribute__((always_inline)) {
-    const int k0 = kb + t * KU + 32 * h;
-    return k0 < it.q.st || k0 + 31 > low;
-  };
   auto hidden = [&](int b, int key) __attribute__((always_inline)) { return key > lim[b] || key < it.q.st; };
   auto apply_mask = [&](int t, int h, f32x16 (&x)[RB]) __attribute__((always_inline)) {
+    const int k0 = kb + t * KU + 32 * h;
+    if (k0 >= it.q.st && k0 + 31 <= low) return;
 #pragma unroll
     for (int b = 0; b < RB; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        x[b][r] = hidden(b, kb + t * KU + 32 * h + (r & 3) + 8 * (r >> 2) + 4 * hi) ? -INFINITY : x[b][r];
+        x[b][r] = hidden(b, k0 + (r & 3) + 8 * (r >> 2) + 4 * hi) ? -INFINITY : x[b][r];
   };
-  auto maxima = [&](const f32x16 (&x)[RB]) __attribute__((always_inline)) {
+  auto maxima = [&](int h, const f32x16 (&x)[RB]) __attribute__((always_inline)) {
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
       float y = x[b][0];
 #pragma unroll
       for (int r = 1; r < 16; ++r) y = fmaxf(y, x[b][r]);
-      mx[b] = y;
+      mx[h][b] = y;
     }
   };
-  auto vfrag = [&](const char* vl, int c, int u) __attribute__((always_inline)) {
-    const int G = lane >> 4, li = lane & 15;
-    const int r1 = 16 * u + 4 * hi + (li >> 2), r2 = r1 + 8;
-    const int ch = 4 * c + 2 * (G & 1) + ((li & 3) >> 1), h8 = (li & 1) << 3;
-    const i16x4 x = read_tr(vl + r1 * ROWB + ((ch ^ swz<D>(r1)) << 4) + h8);
-    const i16x4 y = read_tr(vl + r2 * ROWB + ((ch ^ swz<D>(r2)) << 4) + h8);
-    return i16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-  };
-
-  // tiles that some row of the workgroup sees in part; whether one holds values that are not finite (flags, by V buffer)
+  // tiles that some row of the workgroup sees in part; whether one holds values that are not finite
   const int low0 = a.causal ? it.q.kv - it.q.n + fdiv(R0, a.g) : it.q.kv - 1;
   auto edge = [&](int t) __attribute__((always_inline)) { return kb + t * KU < it.q.st || kb + t * KU + KU - 1 > low0; };
-  auto look = [&](const char* vl) __attribute__((always_inline)) {
+  auto look = [&](int t, const char* vl) __attribute__((always_inline)) {
     if (threadIdx.x == 0) found = 0;
     sync_lds();
+    const int key = kb + t * KU + wrow + lkey[1];
     bool odd = false;
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const u32x4 x = *reinterpret_cast<const u32x4*>(vl + (wrow + i * RPL) * ROWB + lane * 16);
+    for (int p = 0; p < NL; ++p) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(vl + (4 * p + wave) * 1024 + lane * 16);
 #pragma unroll
       for (int e = 0; e < 4; ++e) odd = odd || (x[e] & F::EXP) == F::EXP || (x[e] >> 16 & F::EXP) == F::EXP;
     }
-    if (odd) found = 1;
+    if (odd) atomicOr(&found, key < ke && key >= it.q.st ? 3 : 1);  // 2: at a key that some row may see
     sync_lds();
-    return found != 0;
+    return found;
   };
-
-  At ak{}, av{};  // of K(j + 1) / V(j + 1) at the start of step j
-  if (n > 0) {
-    if constexpr (P16) {
-      pbase = fdiv(kb + wrow, a.ps);
-      if (pbase > lastp) pbase = lastp;
-      pv = clampp(bt[min(pbase + lane, lastp)]);
-      pn = bt[min(pbase + 64 + lane, lastp)];
-    } else {
-      lookup(kb);
-    }
-    At a0{};
-    place(0, a0);
-    fetch(kc, a0, K0);
-    fetch(vc, a0, V0);
-    if (n > 1) {
-      place(1, ak);
-      fetch(kc, ak, K1);
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    sync_lds();
-    scores(K0, 0, s[0]);
-    if (masked(0, 0)) apply_mask(0, 0, s[0]);
-    maxima(s[0]);
-#pragma unroll
-    for (int b = 0; b < RB; ++b) m[b] = fmaxf(NONE, fmaxf(mx[b], other_half(mx[b])) * a.cs);
-  }
-
   // A masked key has p = 0, but 0 times an infinity or NaN in its value would reach the row all the same.  Where a tile
-  // that some row sees in part holds such values (rare), they become zeros in LDS; which sums rows that see them
-  // get +infinity or -infinity into (NaN: both) is found by a product with the mask and kept until the end.
+  // that some row sees in part holds such values, they become zeros in LDS.  Where rows see them (rare, and slow:
+  // key by key), which of their sums get +infinity or -infinity (NaN: both) is kept until the end.
   bool anyinf = false;
-  auto mend = [&](int j, char* vl) __attribute__((always_inline)) {
-    if (!anyinf)
-      for (int i = 0; i < RB * DC; ++i) inf[wave][i][lane] = 0;
-    anyinf = true;
+  auto mend = [&](int j, char* vl, bool seen) __attribute__((always_inline)) {
+    if (seen) {
+      if (!anyinf)
+        for (int i = 0; i < RB * DC; ++i) inf[wave][i][lane] = 0;
+      anyinf = true;
 #pragma nounroll
-    for (int c = 0; c < DC; ++c)
+      for (int key = 0; key < KU; ++key)
 #pragma unroll
-      for (int b = 0; b < RB; ++b) {
-        f32x16 up, dn;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) up[r] = dn[r] = 0.f;
+        for (int b = 0; b < RB; ++b)
+          if (!hidden(b, kb + j * KU + key)) {
 #pragma nounroll
-        for (int u = 0; u < 4; ++u) {
-          v8 fin, isup, isdn, seen;
-          split_values<T>(vfrag(vl, c, u), fin, isup, isdn);
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            seen[i] = hidden(b, kb + j * KU + 16 * u + 4 * hi + (i & 3) + 8 * (i >> 2)) ? (T)0.f : (T)1.f;
-          up = F::mma(isup, seen, up);
-          dn = F::mma(isdn, seen, dn);
-        }
-        int bits = 0;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) bits |= (up[r] > 0.f ? 1 << r : 0) | (dn[r] > 0.f ? 65536 << r : 0);
-        inf[wave][c * RB + b][lane] |= bits;
-      }
-    sync_lds();
+            for (int r = 0; r < DC * 16; ++r) {  // column of O's register r
+              const int d = 32 * (r >> 4) + (r & 3) + 8 * (r >> 2 & 3) + 4 * hi, q = d >> 3 & 3, k16 = key & 15;
+              const unsigned v = *reinterpret_cast<const unsigned short*>(vl + (4 * (d >> 5) + (key >> 4)) * 1024 + q * 256 +
+                                                                          (k16 ^ (q << 2)) * 16 + (d & 7) * 2);
+              if ((v & F::EXP) == F::EXP) {
+                const int up = (v & F::MAN) || !(v & 0x8000), dn = (v & F::MAN) || (v & 0x8000);
+                inf[wave][(r >> 4) * RB + b][lane] |= (up | dn << 16) << (r & 15);
+              }
+            }
+          }
+      sync_lds();
+    }
 #pragma nounroll
-    for (int i = 0; i < NL; ++i) {
-      i16x8* x = reinterpret_cast<i16x8*>(vl + (wrow + i * RPL) * ROWB + lane * 16);
+    for (int p = 0; p < NL; ++p) {
+      i16x8* x = reinterpret_cast<i16x8*>(vl + (4 * p + wave) * 1024 + lane * 16);
       v8 fin, isup, isdn;
       split_values<T>(*x, fin, isup, isdn);
       *x = __builtin_bit_cast(i16x8, fin);
     }
     sync_lds();
   };
-  // O taken out of the way when a maximum grew too much: acc = acc * alpha + O * alpha, O = 0.  In memory, and rare:
-  // vector registers have no room for O, and the matrix unit's own can only be added to.
+  // O taken out of the way when a maximum grew too much: acc = (acc + O) * alpha, O = 0.  In memory, and rare: vector
+  // registers have no room for O, and the matrix unit's own can only be added to.
   volatile float acc[RB * DC * 16], out[RB * DC * 16];
   bool flushed = false;
   auto flush = [&]() __attribute__((always_inline)) {
+    settle();
 #pragma unroll
     for (int b = 0; b < RB; ++b)
 #pragma unroll
@@ -546,93 +544,165 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
-      const float mn = fmaxf(m[b], mx[b]);
+      const float mn = fmaxf(m[b], fmaxf(mx[0][b], mx[1][b]));
       const float alpha = __builtin_amdgcn_exp2f(m[b] - mn);
       m[b] = mn;
       l[b] *= alpha;
+#pragma nounroll
       for (int i = 0; i < DC * 16; ++i) {
         const int e = b * DC * 16 + i;
         const float old = flushed ? acc[e] : 0.f;
         acc[e] = (old + out[e]) * alpha;
       }
     }
-#pragma unroll
-    for (int b = 0; b < RB; ++b)
-#pragma unroll
-      for (int c = 0; c < DC; ++c)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[b][c][r] = 0.f;
+    clear_o();
     flushed = true;
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), here and not on the path that goes around
   };
-  // half h of tile j: x its scores, y those of the next half (nk: its K image; more: there is one)
-  auto half = [&](int j, auto hc, const char* nk, const char* vl, bool more, f32x16 (&x)[RB], f32x16 (&y)[RB])
-                  __attribute__((always_inline)) {
-    constexpr int H = decltype(hc)::value;
-    // raise the maxima where they grew too much
-    bool grow = false;
+
+  At ak{}, av{};  // of K(j + 1) / V(j + 1) at the start of step j
+  if (n > 0) {
+    if constexpr (P16) {
+      pbase = min(fdiv(kb + wrow, a.ps), lastp);
+      pv = clampp(bt[min(pbase + lane, lastp)]);
+      pn = bt[min(pbase + 64 + lane, lastp)];
+    } else {
+      lookup(kb);
+    }
+    At a0{};
+    place(0, a0);
+    fetch(kc, a0, 0, K0);
+    fetch(vc, a0, 1, V0);
+    if (n > 1) {
+      place(1, ak);
+      fetch(kc, ak, 0, K1);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    sync_lds();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      scores(K0, h, s[0][h]);
+      if (edge(0)) apply_mask(0, h, s[0][h]);
+      maxima(h, s[0][h]);
+    }
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
-      mx[b] = fmaxf(mx[b], other_half(mx[b])) * a.cs;
-      grow = grow || mx[b] > m[b] + F::GROW;
+      const float y = fmaxf(mx[0][b], mx[1][b]);
+      m[b] = fmaxf(NONE, fmaxf(y, other_half(y)) * a.cs);
     }
-    if (__ballot(grow)) flush();
-    __builtin_amdgcn_sched_barrier(0);
-    // the next half's scores beside this half's exponentials
-    scores(nk, H ^ 1, y);  // (behind the last half: of what is there, and not used)
+    sync_lds();  // every wave has read K(0): K(2) takes its place
+  }
+
+  // half H of tile j: x its scores; y those of the same half of tile j + 1, from the K image kl.  Written in the order
+  // in which it is to run, fenced slot by slot: a product, then what the vector unit does while it runs, with
+  // fragments read two products' time ahead (kf: the first two are on their way).  left to itself the compiler puts
+  // all products first.
+  auto half = [&](int j, auto hc, const char* kl, const char* vl, f32x16 (&x)[RB], f32x16 (&y)[RB], v8 (&kf)[3])
+                  __attribute__((always_inline)) {
+    constexpr int H = decltype(hc)::value;
+    constexpr int PE = 16 / KS > 0 ? 16 / KS : 1;  // scores of a slot
     v8 pt[RB][2];
+    i16x8 vf[3];
 #pragma unroll
-    for (int b = 0; b < RB; ++b)
+    for (int ks = 0; ks < KS; ++ks) {
+      if (ks + 2 < KS) kf[(ks + 2) % 3] = kfrag(kl, H, ks + 2);
+      if (ks >= KS - 2) vf[ks - (KS - 2)] = vfrag(vl, 0, 2 * H + ks - (KS - 2));
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(x[b][r], a.cs, -m[b]));
-        x[b][r] = p;
-        pt[b][r >> 3][r & 7] = (T)p;  // (rounded to nearest: the matrix unit's operand; the sums keep fp32)
+      for (int b = 0; b < RB; ++b) {
+        if (ks == 0) {
+          f32x16 z;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) z[r] = 0.f;
+          y[b] = F::mma(kf[0], qf[b][0], z);
+        } else {
+          y[b] = F::mma(kf[ks % 3], qf[b][ks], y[b]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < PE; ++i) {
+          const int e = (ks * RB + b) * PE + i, eb = e / 16, r = e % 16;
+          const float p = __builtin_amdgcn_exp2f(fmaf(x[eb][r], a.cs, -m[eb]));
+          x[eb][r] = p;
+          pt[eb][r >> 3][r & 7] = (T)p;  // (rounded to nearest: the matrix unit's operand; the sums keep fp32)
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-    // (here, not where they are used: the exponentials belong beside the scores' products)
+    }
+    // (behind the last tile y is what was there, and not used)
 #pragma unroll
     for (int b = 0; b < RB; ++b)
 #pragma unroll
       for (int u = 0; u < 2; ++u) asm volatile("" : "+v"(pt[b][u]));
     __builtin_amdgcn_sched_barrier(0);
-    if (more && masked(j + H, H ^ 1)) apply_mask(j + H, H ^ 1, y);
+    if (edge(j + 1)) apply_mask(j + 1, H, y);
+    constexpr int SL = 2 * DC, SE = RB * 16 / (SL * RB) > 0 ? 16 / SL : 1;  // slots; sums and maxima of one
+    float t[RB];
 #pragma unroll
-    for (int c = 0; c < DC; ++c)
+    for (int b = 0; b < RB; ++b) t[b] = y[b][0];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const v8 v = __builtin_bit_cast(v8, vfrag(vl, c, 2 * H + u));
+    for (int i = 0; i < SL; ++i) {
+      if (i + 2 < SL) vf[(i + 2) % 3] = vfrag(vl, (i + 2) >> 1, 2 * H + ((i + 2) & 1));
+      if (H == 0 && i >= SL - 2) kf[i - (SL - 2)] = kfrag(kl, 1, i - (SL - 2));
 #pragma unroll
-        for (int b = 0; b < RB; ++b) o[b][c] = F::mma(v, pt[b][u], o[b][c]);
+      for (int b = 0; b < RB; ++b) {
+        F::acc(o[b][i >> 1], __builtin_bit_cast(v8, vf[i % 3]), pt[b][i & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < SE; ++k) {
+          const int e = (i * RB + b) * SE + k, eb = e / 16, r = e % 16;
+          if (e < RB * 16) {
+            l[eb] += x[eb][r];
+            t[eb] = fmaxf(t[eb], y[eb][r]);
+          }
+        }
+        const int pb = (i * RB + b) * SE / 16 % RB;
+        asm volatile("" : "+v"(l[pb]), "+v"(t[pb]));  // (here, not where they are used)
+        __builtin_amdgcn_sched_barrier(0);
       }
+    }
 #pragma unroll
-    for (int b = 0; b < RB; ++b)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) l[b] += x[b][r];
-    maxima(y);
+    for (int b = 0; b < RB; ++b) mx[H][b] = t[b];
   };
-  auto step = [&](int j, char* k0, char* k1, char* v0, char* v1) __attribute__((always_inline)) {
-    // V(j + 1) lies where K(j + 1) did, and takes the place of V(j - 1)
+  using H0 = std::integral_constant<int, 0>;
+  using H1 = std::integral_constant<int, 1>;
+  auto step = [&](int j, char* k0, char* k1, char* v0, char* v1, f32x16 (&x)[2][RB], f32x16 (&y)[2][RB])
+                  __attribute__((always_inline)) {
+    // V(j + 1) lies where K(j + 1) did and takes the place of V(j - 1); K(j + 2) that of K(j)
     av = ak;
-    if (j + 1 < n) fetch(vc, av, v1);
-    if (j + 2 < n) place(j + 2, ak);
-    if (edge(j) && look(v0)) mend(j, v0);
-    half(j, std::integral_constant<int, 0>{}, k0, v0, true, s[0], s[1]);
-    // K(j + 1) is there (behind it: only V(j + 1) and page numbers), and every wave has read K(j)
-    if (j + 1 < n) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
-    sync_lds();
-    if (j + 2 < n) fetch(kc, ak, k0);
-    half(j, std::integral_constant<int, 1>{}, k1, v0, j + 1 < n, s[1], s[0]);
-    // V(j + 1) is there
-    if (j + 2 < n)
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
-    else
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (j + 1 < n) fetch(vc, av, 1, v1);
+    if (j + 2 < n) {
+      place(j + 2, ak);
+      fetch(kc, ak, 0, k0);
+    }
+    // raise the maxima where they grew too much
+    bool grow = false;
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) mx[h][b] = fmaxf(mx[h][b], other_half(mx[h][b])) * a.cs;
+      grow = grow || fmaxf(mx[0][b], mx[1][b]) > m[b] + F::GROW;
+    }
+    if (__ballot(grow)) flush();
+    if (edge(j)) {
+      const int odd = look(j, v0);
+      if (odd) mend(j, v0, odd & 2);
+    }
+    v8 kf[3];
+    kf[0] = kfrag(k1, 0, 0);
+    kf[1] = kfrag(k1, 0, 1);
+    half(j, H0{}, k1, v0, x[0], y[0], kf);
+    half(j, H1{}, k1, v0, x[1], y[1], kf);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     sync_lds();
   };
-  for (int j = 0; j < n; j += 2) {
-    step(j, K0, K1, V0, V1);
-    if (j + 1 < n) step(j + 1, K1, K0, V1, V0);
+  int j = 0;
+  for (; j + 1 < n; j += 2) {  // (a condition on the second step would cost a move of all of O a turn)
+    step(j, K0, K1, V0, V1, s[0], s[1]);
+    step(j + 1, K1, K0, V1, V0, s[1], s[0]);
   }
+  if (j < n) step(j, K0, K1, V0, V1, s[0], s[1]);
 
+  settle();
   // Rows through LDS (the tiles' room: 32 rows of D floats a wave, their 16-byte chunks turned by the row), stored 16
   // bytes a lane.
   float* st = reinterpret_cast<float*>(wave == 0 ? K0 : wave == 1 ? K1 : wave == 2 ? V0 : V1);
@@ -640,6 +710,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
     const float L = l[b] + other_half(l[b]);
+    const int lrow = lane / CH, lcol = (lane % CH) * 8;
 #pragma unroll
     for (int c = 0; c < DC; ++c)
 #pragma unroll
