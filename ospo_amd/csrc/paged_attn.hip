@@ -260,6 +260,15 @@ __device__ __forceinline__ i16x4 read_tr(const char* src) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_AS i16x4*)src);
 }
 
+// all loads and LDS-DMA but the last N done (a wait that the compiler sees: what it believes to be in flight, it waits
+// for again, and then for all of it)
+template <int N = 0>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x0f70);  // vmcnt(N)
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);  // (products on what was loaded stay behind it)
+}
 // barrier of the workgroup behind this wave's LDS accesses (loads and LDS-DMA from memory stay in flight)
 __device__ __forceinline__ void sync_lds() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -557,7 +566,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     }
     clear_o();
     flushed = true;
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), here and not on the path that goes around
+    wait_loads();  // here, and not on the path that goes around
   };
 
   At ak{}, av{};  // of K(j + 1) / V(j + 1) at the start of step j
@@ -577,7 +586,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       place(1, ak);
       fetch(kc, ak, 0, K1);
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    wait_loads();
     sync_lds();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -592,6 +601,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     }
     sync_lds();  // every wave has read K(0): K(2) takes its place
   }
+  wait_loads();  // (nothing is in flight: the compiler sees a way around the wait above, and would wait in the loop)
 
   // half H of tile j: x its scores; y those of the same half of tile j + 1, from the K image kl.  Written in the order
   // in which it is to run, fenced slot by slot: a product, then what the vector unit does while it runs, with
@@ -692,7 +702,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     kf[1] = kfrag(k1, 0, 1);
     half(j, H0{}, k1, v0, x[0], y[0], kf);
     half(j, H1{}, k1, v0, x[1], y[1], kf);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    wait_loads();
     sync_lds();
   };
   int j = 0;
@@ -938,6 +948,56 @@ __global__ __launch_bounds__(256) void paged_few_kernel(const PagedArgs a) {
   const int li = lane & 15, vq = (li & 3) >> 1;
   const unsigned va = (unsigned)(uintptr_t)((LDS_AS const char*)vbuf) +
                       (vq * 16 + ((4 * G + (li >> 2)) ^ (vq << 3))) * 16 + (li & 1) * 8;
+  // A masked key has p = 0, but 0 times an infinity or NaN in its value would reach the row all the same: in a tile that
+  // some row sees in part such values become zeros in LDS.  Where rows see them (rare, and slow: key by key), which of
+  // their sums get +infinity or -infinity (NaN: both) is kept until the end: 8 bits for each chain of O.
+  unsigned inf[DC / 4];
+#pragma unroll
+  for (int c = 0; c < DC / 4; ++c) inf[c] = 0;
+  auto mend = [&](int k0, int b) __attribute__((always_inline)) {
+    char* vl = vbuf + b * NW * VB;
+    bool odd = false, seen = false;
+#pragma nounroll
+    for (int p = 0; p < 2 * KS; ++p) {
+      const u32x4 x = *reinterpret_cast<const u32x4*>(vl + p * 1024 + lane * 16);
+      bool here = false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        here = here || (x[e] & Frag<T>::EXP) == Frag<T>::EXP || (x[e] >> 16 & Frag<T>::EXP) == Frag<T>::EXP;
+      const int key = k0 + 16 * (p / KS) + vrow;
+      odd = odd || here;
+      seen = seen || (here && key < ke && key >= it.q.st);
+    }
+    if (!__ballot(odd)) return;
+    if (__ballot(seen)) {
+#pragma nounroll
+      for (int key = 0; key < KT; ++key) {
+        const bool hid = k0 + key > lim || k0 + key < it.q.st;
+#pragma unroll
+        for (int c = 0; c < DC; ++c) {
+          const int q = 2 * (c & 1) + (G >> 1), kk = (key & 15) ^ ((q & 1) << 3);
+          const i16x4 x = *reinterpret_cast<const i16x4*>(vl + ((key >> 4) * KS + (c >> 1)) * 1024 + (q * 16 + kk) * 16 +
+                                                          (G & 1) * 8);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const unsigned v = (unsigned short)x[e];
+            const bool odd1 = !hid && (v & Frag<T>::EXP) == Frag<T>::EXP, nan = v & Frag<T>::MAN;
+            if (odd1 && (nan || !(v & 0x8000))) inf[c >> 2] |= 1u << (8 * (c & 3) + e);
+            if (odd1 && (nan || (v & 0x8000))) inf[c >> 2] |= 16u << (8 * (c & 3) + e);
+          }
+        }
+      }
+    }
+#pragma nounroll
+    for (int p = 0; p < 2 * KS; ++p) {
+      i16x8* x = reinterpret_cast<i16x8*>(vl + p * 1024 + lane * 16);
+      v8 fin, up, dn;
+      split_values<T>(*x, fin, up, dn);
+      *x = __builtin_bit_cast(i16x8, fin);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  };
+
   v8 ka[2][KS], kn[2][KS];
   auto work = [&](int i, int b, v8 (&kf)[2][KS]) __attribute__((always_inline)) {
     const int k0 = kw + i * KU;
@@ -979,6 +1039,7 @@ __global__ __launch_bounds__(256) void paged_few_kernel(const PagedArgs a) {
       }
     l = l * alpha + sum;  // this lane's keys; the lanes of a row are added up at the end
     const unsigned vb = va + b * NW * VB;
+    if (mask) mend(k0, b);
 #pragma unroll
     for (int c4 = 0; c4 < DC; c4 += 4) {
       i16x4 lo[4], hi[4];
@@ -990,52 +1051,41 @@ __global__ __launch_bounds__(256) void paged_few_kernel(const PagedArgs a) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const i16x8 vv = {lo[c][0], lo[c][1], lo[c][2], lo[c][3], hi[c][0], hi[c][1], hi[c][2], hi[c][3]};
-        if (!mask) {
-          o[c4 + c] = Mma16<T>::mma(__builtin_bit_cast(v8, vv), pt, o[c4 + c] * alpha);
-        } else {
-          // a value that some row doesn't see must not reach it, whatever it is: see paged_many_kernel
-          f32x4 x = Mma16<T>::mma(__builtin_bit_cast(v8, vv), pt, f32x4{0.f, 0.f, 0.f, 0.f});
-          float bad = 0.f;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) bad = fmaf(x[e], 0.f, bad);
-          if (__ballot(bad != 0.f)) {
-            v8 fin, up, dn, seen;
-            split_values<T>(vv, fin, up, dn);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int key = k0 + 16 * (e >> 2) + 4 * G + (e & 3);
-              seen[e] = key > lim || key < it.q.st ? (T)0.f : (T)1.f;
-            }
-            const f32x4 z = {0.f, 0.f, 0.f, 0.f};
-            x = Mma16<T>::mma(fin, pt, z);
-            const f32x4 u = Mma16<T>::mma(up, seen, z), w = Mma16<T>::mma(dn, seen, z);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if (u[e] > 0.f) x[e] += INFINITY;
-              if (w[e] > 0.f) x[e] -= INFINITY;
-            }
-          }
-          o[c4 + c] = o[c4 + c] * alpha + x;
-        }
+        o[c4 + c] = Mma16<T>::mma(__builtin_bit_cast(v8, vv), pt, o[c4 + c] * alpha);
       }
     }
   };
   // operations of one issue() behind which a wait may stop: the V pieces and K loads of the next tile
   constexpr int AHEAD = 4 * KS;
-  auto step = [&](int i, int b, v8 (&kf)[2][KS], v8 (&kx)[2][KS]) __attribute__((always_inline)) {
-    if (i + 1 < n) {
-      issue(i + 1, vbuf + (b ^ 1) * NW * VB, kx);
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(AHEAD) : "memory");
-    } else {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    }
-    work(i, b, kf);
-  };
+  // (the last tiles apart: in one loop the compiler sees a way around the waits, and would wait for all that is in flight)
+  char* const v1 = vbuf + NW * VB;
+  int i = 0;
   if (n > 0) issue(0, vbuf, ka);
-  for (int i = 0; i < n; i += 2) {
-    step(i, 0, ka, kn);
-    if (i + 1 < n) step(i + 1, 1, kn, ka);
+  for (; i + 2 < n; i += 2) {
+    issue(i + 1, v1, kn);
+    wait_loads<AHEAD>();
+    work(i, 0, ka);
+    issue(i + 2, vbuf, ka);
+    wait_loads<AHEAD>();
+    work(i + 1, 1, kn);
   }
+  if (i + 1 < n) {
+    issue(i + 1, v1, kn);
+    wait_loads<AHEAD>();
+    work(i, 0, ka);
+    wait_loads();
+    work(i + 1, 1, kn);
+  } else if (i < n) {
+    wait_loads();
+    work(i, 0, ka);
+  }
+#pragma unroll
+  for (int c = 0; c < DC; ++c)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (inf[c >> 2] >> (8 * (c & 3)) & 1u << e) o[c][e] += INFINITY;
+      if (inf[c >> 2] >> (8 * (c & 3)) & 16u << e) o[c][e] -= INFINITY;
+    }
   l = sum_groups(l);
 
   // join the waves and store
