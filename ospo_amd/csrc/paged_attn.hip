@@ -44,9 +44,10 @@ struct PagedArgs {
   int qvec, ovec;  // q rows and o rows allow 16-byte access
   int slots;       // workgroups that run at once: what a split aims for
   int split;       // 0: every item is one chunk
-  long items;      // of the launch (an upper bound of those there are)
-  float* ws;       // partial O [item][BM][D], then (m, l) [item][BM][2]
-  long ws_ml;      // offset of the latter, floats
+  long items, pairs;  // workgroups of the two launches: upper bounds
+  int* plan;       // number of (tile, head) pairs, then from PLAN_HEAD on their records for the joining launch
+  float* ws;       // partial O [item][BM][D]
+  float* ml;       // (m, l) [item][BM][2]
 };
 
 // ---------------------------------------------------------------- items
@@ -102,11 +103,12 @@ __device__ __forceinline__ LaneSeq lane_seq(const PagedArgs& a, int s) {
   }
   return r;
 }
-// Key blocks of a chunk.  With L = all work / slots: where the tiles alone fill the slots, chunks of at most L / 4
-// even out the last round (with many tiles, only sequences longer than L are cut); where they do not, the smallest
-// chunk that keeps one round.
+// Key blocks of a chunk.  With L = all work / slots: where the tiles alone fill the slots, chunks of at most L / 4, but
+// four blocks at least, even out the last round (with many tiles, only sequences longer than L are cut).  Where they do not, one round:
+// of L, the smallest chunk that might do, and of the smaller of two that do (every tile cut as the longest may be;
+// the work over the slots that the tiles leave), the first of four steps from one to the other that fits.
 template <int BM, int KU>
-__device__ __forceinline__ int pick_chunk(const PagedArgs& a, int lane, const LaneSeq& first) {
+__device__ __forceinline__ unsigned pick_chunk(const PagedArgs& a, int lane, const LaneSeq& first) {
   if (!a.split) return 0x7fffffff;
   float total = 0.f;
   int base = 0, most = 1;
@@ -116,76 +118,96 @@ __device__ __forceinline__ int pick_chunk(const PagedArgs& a, int lane, const La
     base += sum_i(q.tiles);
     most = max(most, max_i(q.tiles ? q.units : 0));
   }
-  base *= a.Hk;
-  const float L = total * (float)a.Hk / (float)a.slots;
-  if (base > a.slots) return (int)fminf((float)most, ceilf(base >= 4 * a.slots ? L : 0.25f * L));
-  int C = (int)fminf((float)most, fmaxf(1.f, ceilf(L)));
-  while (C < most) {
+  base = max(1, base * a.Hk);
+  total *= (float)a.Hk;
+  const float L = total / (float)a.slots;
+  if (base > a.slots) return (unsigned)fmaxf(4.f, fminf((float)most, ceilf(base >= 4 * a.slots ? L : 0.25f * L)));
+  const float lo = fmaxf(1.f, ceilf(L));
+  const unsigned times = (unsigned)a.slots / (unsigned)base;
+  float hi = (float)(((unsigned)most + times - 1) / times);
+  if (a.slots > base) hi = fminf(hi, ceilf(1.00001f * total / (float)(a.slots - base)) + 1.f);
+  hi = fmaxf(lo, hi) + (most > 1 << 22 ? 4.f : 0.f);  // (sums and counts of that size are rounded)
+  for (int i = 0; i < 4; ++i) {
+    const unsigned C = (unsigned)(lo + (hi - lo) * 0.25f * (float)i);
     int n = 0;
     for (int s0 = 0; s0 < a.S; s0 += 64) {
       const LaneSeq q = s0 ? lane_seq<BM, KU>(a, s0 + lane) : first;
-      n += sum_i(q.tiles * (int)(((unsigned)q.units + C - 1) / (unsigned)C));
+      n += sum_i(q.tiles * (int)(((unsigned)q.units - 1) / C + 1));
     }
-    if (n * a.Hk <= a.slots) break;
-    C += (C + 7) / 8;
+    if (n * a.Hk <= a.slots) return C;
+    if (hi - lo < 1.f) break;
   }
-  return C;
+  return (unsigned)hi;
 }
 
 struct Item {
   Seq q;
   int seq, tile, head, chunk, nch, cs, u0, units;
-  int first, step;  // item index of chunk 0 of this (tile, head); its chunks are `step` apart
+  int step;  // the item indices of a (tile, head)'s chunks are this far apart
+  int pair;  // number of the (tile, head)
 };
 // Order of a sequence's items: heads fastest over the XCDs (hb = largest power of two <= 8 that divides Hk, so a
 // key/value head stays in its XCDs' L2), then chunks, then tiles from the last (the longest rows first), then the
-// remaining heads.  PAIR: item number `id` counts (tile, head) pairs (the joining launch).
-template <int BM, int KU, bool PAIR>
+// remaining heads.  Item 0's workgroup also notes how many (tile, head) pairs there are.
+template <int BM, int KU>
 __device__ __forceinline__ bool find_item(const PagedArgs& a, int id, int lane, Item& it) {
   const LaneSeq lead = lane_seq<BM, KU>(a, lane);
-  const unsigned C = (unsigned)max(1, pick_chunk<BM, KU>(a, lane, lead));
-  int before = 0, ibefore = 0;
+  const unsigned C = pick_chunk<BM, KU>(a, lane, lead);
+  int before = 0, pairs = 0;
+  bool got = false;
   for (int s0 = 0; s0 < a.S; s0 += 64) {
     const LaneSeq q = s0 ? lane_seq<BM, KU>(a, s0 + lane) : lead;
     const int nch = (int)(((unsigned)q.units - 1) / C) + 1;
-    const int pairs = q.tiles * a.Hk;
-    const int items = scan_add(pairs * nch);
-    const int mine = PAIR ? scan_add(pairs) : items;
-    const unsigned long long b = __ballot(id - before < mine);
-    if (b) {
+    const int own = q.tiles * a.Hk, mine = own * nch;
+    const int upto = scan_add(mine), pupto = scan_add(own);
+    const unsigned long long b = __ballot(id - before < upto);
+    if (b && !got) {
       const int w = __ffsll(b) - 1;
       it.seq = s0 + w;
       it.q.q0 = lane_of(q.q.q0, w), it.q.n = lane_of(q.q.n, w);
       it.q.kv = lane_of(q.q.kv, w), it.q.st = lane_of(q.q.st, w);
       it.units = lane_of(q.units, w), it.nch = lane_of(nch, w);
       const unsigned tiles = (unsigned)lane_of(q.tiles, w);
-      const int np = lane_of(pairs, w);
-      const unsigned at = (unsigned)(id - before - (lane_of(mine, w) - (PAIR ? np : np * it.nch)));
-      const int ibase = ibefore + lane_of(items, w) - np * it.nch;
+      const unsigned at = (unsigned)(id - before - lane_of(upto - mine, w));
       const int hb = min(8, a.Hk & -a.Hk), sh = __ffs(hb) - 1;
-      const unsigned hl = at & (hb - 1), z = at >> sh;
-      const unsigned per = PAIR ? tiles : tiles * it.nch;
-      const unsigned hh = z / per, x = z - hh * per;
-      const unsigned tx = PAIR ? x : x / it.nch;
-      it.head = (int)(hh * hb + hl);
+      const unsigned z = at >> sh, per = tiles * it.nch;
+      const unsigned hh = z / per, x = z - hh * per, tx = x / it.nch;
+      it.head = (int)((hh << sh) + (at & (hb - 1)));
       it.tile = (int)(tiles - 1 - tx);
-      it.chunk = PAIR ? 0 : (int)(x - tx * it.nch);
+      it.chunk = (int)(x - tx * it.nch);
       it.cs = (int)(((unsigned)it.units + it.nch - 1) / it.nch);
       it.u0 = it.q.st / KU;
-      it.first = ibase + (int)(((hh * tiles + tx) * it.nch << sh) + hl);
       it.step = hb;
-      return true;
+      it.pair = pairs + lane_of(pupto - own, w) + (int)(((hh * tiles + tx) << sh) + (at & (hb - 1)));
+      got = true;
+      if (id > 0) return true;
     }
-    before += lane_of(mine, 63);
-    ibefore += lane_of(items, 63);
+    before += lane_of(upto, 63);
+    pairs += lane_of(pupto, 63);
   }
-  return false;
+  if (id == 0 && a.split && threadIdx.x == 0) a.plan[0] = pairs;
+  return got;
 }
 // one past the last key that any row of the tile sees
 __device__ __forceinline__ int tile_end(const PagedArgs& a, const Item& it, int BM) {
   if (!a.causal) return it.q.kv;
   const int last = min((it.tile + 1) * BM, it.q.n * (int)a.g.d) - 1;
   return max(0, it.q.kv - it.q.n + fdiv(last, a.g) + 1);
+}
+
+// What the joining launch needs to know of a (tile, head): how many chunks to join (0: none), its first item.
+struct Record {
+  int chunks, first, step, q0, head, row0, rows;
+};
+constexpr int PLAN_HEAD = 8, RECORD = 8;  // ints
+template <int BM, int KU>
+__device__ __forceinline__ void note(const PagedArgs& a, const Item& it, int end) {
+  if (!a.split || it.chunk > 0 || threadIdx.x) return;
+  const int left = min(end, (it.u0 + it.units) * KU) - it.u0 * KU;
+  const int n = left > 0 ? ((left + KU - 1) / KU + it.cs - 1) / it.cs : 1;  // chunks that have keys (one writes if none has)
+  Record r{it.nch > 1 ? n : 0, (int)blockIdx.x, it.step, it.q.q0, it.head, it.tile * BM,
+           min(BM, it.q.n * (int)a.g.d - it.tile * BM)};
+  if (it.pair < a.pairs) *reinterpret_cast<Record*>(a.plan + PLAN_HEAD + (long)it.pair * RECORD) = r;
 }
 
 // ---------------------------------------------------------------- types
@@ -254,6 +276,12 @@ __device__ __forceinline__ int swz(int r) {
 // 16 bytes a lane from global memory to LDS (wave-uniform destination + 16 lane), without registers
 __device__ __forceinline__ void dma16(const void* src, char* dst) {
   __builtin_amdgcn_global_load_lds(src, (LDS_AS void*)dst, 16, 0, 0);
+}
+// The same from a uniform base by a 32-bit byte offset a lane and a uniform one more.  (While pieces of the form above are
+// in flight the compiler lets every LDS read wait for all that went before it.)
+__device__ __forceinline__ void dma16_from(const void* base, char* dst, int voff, int soff) {
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7fffffff, 0x00020000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (LDS_AS void*)dst, 16, voff, soff, 0, 0);
 }
 // transposed read: a group of 16 lanes reads 4 rows x 16 columns, lane i gets column i
 __device__ __forceinline__ i16x4 read_tr(const char* src) {
@@ -335,13 +363,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   const int hi = lane >> 5, l32 = lane & 31;
 
   Item it;
-  if (!find_item<BM, KU, false>(a, blockIdx.x, lane, it)) return;
+  if (!find_item<BM, KU>(a, blockIdx.x, lane, it)) return;
   const int R = it.q.n * (int)a.g.d;
   const int ub = it.u0 + it.chunk * it.cs;
   const int kb = ub * KU;
-  const int ke = min(min(ub + it.cs, it.u0 + it.units) * KU, tile_end(a, it, BM));
+  const int end = tile_end(a, it, BM);
+  const int ke = min(min(ub + it.cs, it.u0 + it.units) * KU, end);
   const bool part = it.nch > 1;
-  if (part && it.chunk > 0 && kb >= ke) return;  // the joining launch counts the same chunks
+  note<BM, KU>(a, it, end);
+  if (part && it.chunk > 0 && kb >= ke) return;
   const int R0 = it.tile * BM, row0 = R0 + wave * 32 * RB;
 
   // rows of this lane: row0 + 32 b + l32 (rows behind the last repeat it and are not stored)
@@ -424,17 +454,23 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
         const int key = min(k0 + wrow + lkey[i], ke - 1);
         at.v[i] = (long)clampp(pg[i]) * a.c_ps + (long)(key - fdiv(key, a.ps) * (int)a.ps.d) * a.c_ts + 8 * q4;
       }
-      if (t + 1 < n) lookup(k0 + KU);
+      lookup(k0 + KU);
     }
   };
   const int loff[2] = {lkey[0] * (int)a.c_ts + 8 * q4, lkey[1] * (int)a.c_ts + 8 * q4};
+  auto piece = [&](const T* base, const At& at, int i, char* buf, int p) __attribute__((always_inline)) {
+    if constexpr (P16)
+      dma16_from(base + at.u, buf + (4 * p + wave) * 1024, 2 * loff[i], 64 * p);
+    else
+      dma16(base + at.v[i] + 32 * p, buf + (4 * p + wave) * 1024);
+  };
   auto fetch = [&](const T* base, const At& at, int i, char* buf) __attribute__((always_inline)) {
-    const T* src = P16 ? base + at.u + loff[i] : base + at.v[i];
 #pragma unroll
-    for (int p = 0; p < NL; ++p) dma16(src + 32 * p, buf + (4 * p + wave) * 1024);
+    for (int p = 0; p < NL; ++p) piece(base, at, i, buf, p);
   };
 
-  // ---- fragments
+  // ---- fragments: read PF slots of RB products ahead of their use
+  constexpr int PF = 3;
   const int kat = (l32 >> 4) * 1024 + hi * 256 + (l32 & 15) * 16;
   auto kfrag = [&](const char* kl, int h, int ks) __attribute__((always_inline)) {
     return *reinterpret_cast<const v8*>(kl + kat + (ks >> 1) * 4096 + (ks & 1) * 512 + h * 2048);
@@ -566,7 +602,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     }
     clear_o();
     flushed = true;
-    wait_loads();  // here, and not on the path that goes around
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0), here and not on the path that goes around
   };
 
   At ak{}, av{};  // of K(j + 1) / V(j + 1) at the start of step j
@@ -582,10 +618,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     place(0, a0);
     fetch(kc, a0, 0, K0);
     fetch(vc, a0, 1, V0);
-    if (n > 1) {
-      place(1, ak);
-      fetch(kc, ak, 0, K1);
-    }
+    place(min(1, n - 1), ak);
+    fetch(kc, ak, 0, K1);
     wait_loads();
     sync_lds();
 #pragma unroll
@@ -605,18 +639,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
 
   // half H of tile j: x its scores; y those of the same half of tile j + 1, from the K image kl.  Written in the order
   // in which it is to run, fenced slot by slot: a product, then what the vector unit does while it runs, with
-  // fragments read two products' time ahead (kf: the first two are on their way).  left to itself the compiler puts
-  // all products first.
-  auto half = [&](int j, auto hc, const char* kl, const char* vl, f32x16 (&x)[RB], f32x16 (&y)[RB], v8 (&kf)[3])
-                  __attribute__((always_inline)) {
+  // fragments read PF slots ahead (kf: the first are on their way).  Left to itself the compiler puts all products first.
+  auto half = [&](int j, auto hc, const char* kl, const char* vl, f32x16 (&x)[RB], f32x16 (&y)[RB], v8 (&kf)[PF + 1],
+                  auto&& ahead) __attribute__((always_inline)) {
     constexpr int H = decltype(hc)::value;
     constexpr int PE = 16 / KS > 0 ? 16 / KS : 1;  // scores of a slot
     v8 pt[RB][2];
-    i16x8 vf[3];
+    i16x8 vf[PF + 1];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      if (ks + 2 < KS) kf[(ks + 2) % 3] = kfrag(kl, H, ks + 2);
-      if (ks >= KS - 2) vf[ks - (KS - 2)] = vfrag(vl, 0, 2 * H + ks - (KS - 2));
+      if (ks + PF < KS) kf[(ks + PF) % (PF + 1)] = kfrag(kl, H, ks + PF);
+      const int v = ks - (KS - PF);
+      if (v >= 0) vf[v] = vfrag(vl, v >> 1, 2 * H + (v & 1));
 #pragma unroll
       for (int b = 0; b < RB; ++b) {
         if (ks == 0) {
@@ -625,7 +659,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
           for (int r = 0; r < 16; ++r) z[r] = 0.f;
           y[b] = F::mma(kf[0], qf[b][0], z);
         } else {
-          y[b] = F::mma(kf[ks % 3], qf[b][ks], y[b]);
+          y[b] = F::mma(kf[ks % (PF + 1)], qf[b][ks], y[b]);
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -635,6 +669,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
           x[eb][r] = p;
           pt[eb][r >> 3][r & 7] = (T)p;  // (rounded to nearest: the matrix unit's operand; the sums keep fp32)
         }
+        if (ks % 2 && b == RB - 1) ahead(ks / 2);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -651,11 +686,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     for (int b = 0; b < RB; ++b) t[b] = y[b][0];
 #pragma unroll
     for (int i = 0; i < SL; ++i) {
-      if (i + 2 < SL) vf[(i + 2) % 3] = vfrag(vl, (i + 2) >> 1, 2 * H + ((i + 2) & 1));
-      if (H == 0 && i >= SL - 2) kf[i - (SL - 2)] = kfrag(kl, 1, i - (SL - 2));
+      if (i + PF < SL) vf[(i + PF) % (PF + 1)] = vfrag(vl, (i + PF) >> 1, 2 * H + ((i + PF) & 1));
+      if (H == 0 && i >= SL - PF) kf[i - (SL - PF)] = kfrag(kl, 1, i - (SL - PF));
 #pragma unroll
       for (int b = 0; b < RB; ++b) {
-        F::acc(o[b][i >> 1], __builtin_bit_cast(v8, vf[i % 3]), pt[b][i & 1]);
+        F::acc(o[b][i >> 1], __builtin_bit_cast(v8, vf[i % (PF + 1)]), pt[b][i & 1]);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int k = 0; k < SE; ++k) {
@@ -667,6 +702,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
         }
         const int pb = (i * RB + b) * SE / 16 % RB;
         asm volatile("" : "+v"(l[pb]), "+v"(t[pb]));  // (here, not where they are used)
+        if (i % 2 && b == RB - 1) ahead(NL + i / 2);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -678,12 +714,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   auto step = [&](int j, char* k0, char* k1, char* v0, char* v1, f32x16 (&x)[2][RB], f32x16 (&y)[2][RB])
                   __attribute__((always_inline)) {
     // V(j + 1) lies where K(j + 1) did and takes the place of V(j - 1); K(j + 2) that of K(j)
+    // (behind the last tile: the last again), a piece every other slot of the first half, as a row of them would hold
+    // up the wave
     av = ak;
-    if (j + 1 < n) fetch(vc, av, 1, v1);
-    if (j + 2 < n) {
-      place(j + 2, ak);
-      fetch(kc, ak, 0, k0);
-    }
+    place(min(j + 2, n - 1), ak);
+    auto ahead = [&](int p) __attribute__((always_inline)) {
+      if (p < NL)
+        piece(vc, av, 1, v1, p);
+      else
+        piece(kc, ak, 0, k0, p - NL);
+    };
+    auto none = [](int) {};
     // raise the maxima where they grew too much
     bool grow = false;
 #pragma unroll
@@ -697,11 +738,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       const int odd = look(j, v0);
       if (odd) mend(j, v0, odd & 2);
     }
-    v8 kf[3];
-    kf[0] = kfrag(k1, 0, 0);
-    kf[1] = kfrag(k1, 0, 1);
-    half(j, H0{}, k1, v0, x[0], y[0], kf);
-    half(j, H1{}, k1, v0, x[1], y[1], kf);
+    v8 kf[PF + 1];
+#pragma unroll
+    for (int ks = 0; ks < PF; ++ks) kf[ks] = kfrag(k1, 0, ks);
+    half(j, H0{}, k1, v0, x[0], y[0], kf, ahead);
+    half(j, H1{}, k1, v0, x[1], y[1], kf, none);
     wait_loads();
     sync_lds();
   };
@@ -741,7 +782,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       }
     __builtin_amdgcn_wave_barrier();
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll
+#pragma nounroll  // (once an item: what its code takes to fetch is most of its time)
     for (int i = 0; i < 32 / RPL; ++i) {
       const int lr = i * RPL + lrow, r = row0 + 32 * b + lr;
       const float Lr = __shfl(L, lr, 64), Mr = __shfl(m[b], lr, 64);
@@ -752,7 +793,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
         const long slot = (long)blockIdx.x * BM + (r - R0);
         *reinterpret_cast<f32x4*>(a.ws + slot * D + lcol) = x0;
         *reinterpret_cast<f32x4*>(a.ws + slot * D + lcol + 4) = x1;
-        if (lcol == 0) *reinterpret_cast<f32x2*>(a.ws + a.ws_ml + slot * 2) = f32x2{Mr, Lr};
+        if (lcol == 0) *reinterpret_cast<f32x2*>(a.ml + slot * 2) = f32x2{Mr, Lr};
       } else {
         const int tok = fdiv(r, a.g), hd = it.head * (int)a.g.d + r - tok * (int)a.g.d;
         const float x[8] = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
@@ -766,10 +807,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
 
 // ---------------------------------------------------------------- few rows
 // Up to 16 rows for each sequence and key/value head (single tokens): the keys' bytes bound it.  Four waves share out
-// the key tiles (32 keys each); a wave streams on its own, with no barrier until the end: while it works on a tile,
-// the next one's keys are on their way into registers (they are the A operand of S^T = K Q^T as they lie in
-// memory) and its values into LDS (from where the transposed reads of O^T += V^T P^T take them).  16 x 16 x 32
-// products: a 32-row form would spend twice the exponentials and registers on rows that are not there.
+// the key tiles (32 keys each); a wave streams on its own, with no barrier until the end.  A tile's keys come into
+// registers (as they lie in memory they are the A operand of S^T = K Q^T), its values into LDS, from where the
+// transposed reads of O^T += V^T P^T take them.  16 x 16 x 32 products: a 32-row form would spend twice the
+// exponentials and registers on rows that are not there.  One buffer a wave and three workgroups a CU start
+// sooner than two buffers and two workgroups: 32 sequences of 24 to 640 keys, 32 heads of 128, in 28.9 us instead of 34.3;
+// contexts of 4k to 32k are read at the same 5.1 TB/s.  Four workgroups a CU spill registers (4.4 TB/s).
 //
 // The V image of 16 keys x 32 columns is 1 KiB: [16-byte chunk q][key ^ 8 (q & 1)], so that the transposed reads of
 // half a wave (8 keys x 2 chunks) meet every bank once.
@@ -824,8 +867,12 @@ __device__ __forceinline__ void read_v4(unsigned at, i16x4 (&lo)[4], i16x4 (&hi)
       : "memory");
 }
 
+// workgroups of a CU: what the registers allow without spills
+constexpr int few_per_cu(int D) { return D <= 64 ? 4 : D <= 128 ? 3 : 2; }
+
 template <typename T, int D, bool P16>
-__global__ __launch_bounds__(256) void paged_few_kernel(const PagedArgs a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_per_cu(D)))) void paged_few_kernel(
+    const PagedArgs a) {
   using v8 = typename Frag<T>::v8;
   constexpr int BM = 16, KT = 32, NW = 4, KU = KT * NW;
   constexpr int KS = D / 32;   // d steps of S; also 64-byte column blocks of a row
@@ -833,19 +880,21 @@ __global__ __launch_bounds__(256) void paged_few_kernel(const PagedArgs a) {
   constexpr int VB = KT * D * 2;  // bytes of a V tile
   constexpr int PITCH = pitch_of(D);
   constexpr int OUT = NW * BM * PITCH * 4 + NW * BM * 8;
-  __shared__ __attribute__((aligned(16))) char smem[2 * NW * VB > OUT ? 2 * NW * VB : OUT];
+  __shared__ __attribute__((aligned(16))) char smem[NW * VB > OUT ? NW * VB : OUT];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int G = lane >> 4, l16 = lane & 15;
 
   Item it;
-  if (!find_item<BM, KU, false>(a, blockIdx.x, lane, it)) return;
+  if (!find_item<BM, KU>(a, blockIdx.x, lane, it)) return;
   const int R = it.q.n * (int)a.g.d;
   const int ub = it.u0 + it.chunk * it.cs;
   const int kb = ub * KU;
-  const int ke = min(min(ub + it.cs, it.u0 + it.units) * KU, tile_end(a, it, BM));
+  const int end = tile_end(a, it, BM);
+  const int ke = min(min(ub + it.cs, it.u0 + it.units) * KU, end);
   const bool part = it.nch > 1;
-  if (part && it.chunk > 0 && kb >= ke) return;  // the joining launch counts the same chunks
+  note<BM, KU>(a, it, end);
+  if (part && it.chunk > 0 && kb >= ke) return;
   const int row0 = it.tile * BM;
 
   // this lane's row (rows behind the last repeat it and are not stored)
@@ -906,11 +955,10 @@ __global__ __launch_bounds__(256) void paged_few_kernel(const PagedArgs a) {
     }
   }
 
-  // start tile i: V into LDS buffer `buf`, K into registers
-  auto issue = [&](int i, char* buf, v8 (&kf)[2][KS]) __attribute__((always_inline)) {
+  // where tile i's keys and values lie (K by its own lanes' rows; V: the address is kept until its turn)
+  const T *kp[2], *vp[2];
+  auto place = [&](int i) __attribute__((always_inline)) {
     const int k0 = kw + i * KU;
-    const T* kp[2];
-    const T* vp[2];
     if constexpr (P16) {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -923,26 +971,31 @@ __global__ __launch_bounds__(256) void paged_few_kernel(const PagedArgs a) {
           pn = bt[min(pbase + 64 + lane, lastp)];
         }
         const long off = (long)lane_of(pv, pc - pbase) * a.c_ps + (long)slot * a.c_ts;
-        kp[t] = kc + off + l16 * a.c_ts;
-        vp[t] = vc + off + vrow * a.c_ts;
+        kp[t] = kc + off + l16 * a.c_ts + 8 * G;
+        vp[t] = vc + off + vrow * a.c_ts + 8 * G;
       }
     } else {
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const int kk = min(k0 + 16 * t + l16, ke - 1), kv = min(k0 + 16 * t + vrow, ke - 1);
-        kp[t] = kc + (long)clampp(pg[t]) * a.c_ps + (long)(kk - fdiv(kk, a.ps) * (int)a.ps.d) * a.c_ts;
-        vp[t] = vc + (long)clampp(pg[2 + t]) * a.c_ps + (long)(kv - fdiv(kv, a.ps) * (int)a.ps.d) * a.c_ts;
+        kp[t] = kc + (long)clampp(pg[t]) * a.c_ps + (long)(kk - fdiv(kk, a.ps) * (int)a.ps.d) * a.c_ts + 8 * G;
+        vp[t] = vc + (long)clampp(pg[2 + t]) * a.c_ps + (long)(kv - fdiv(kv, a.ps) * (int)a.ps.d) * a.c_ts + 8 * G;
       }
-      if (i + 1 < n) lookup(k0 + KU);
+      lookup(k0 + KU);
     }
+  };
+  v8 kf[2][KS];
+  auto issue_k = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int p = 0; p < KS; ++p) dma16(vp[t] + 32 * p + 8 * G, buf + (t * KS + p) * 1024);
+      for (int ks = 0; ks < KS; ++ks) kf[t][ks] = *reinterpret_cast<const v8*>(kp[t] + 32 * ks);
+  };
+  auto issue_v = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) kf[t][ks] = *reinterpret_cast<const v8*>(kp[t] + 32 * ks + 8 * G);
+      for (int p = 0; p < KS; ++p) dma16(vp[t] + 32 * p, vbuf + (t * KS + p) * 1024);
   };
 
   const int li = lane & 15, vq = (li & 3) >> 1;
@@ -954,8 +1007,8 @@ __global__ __launch_bounds__(256) void paged_few_kernel(const PagedArgs a) {
   unsigned inf[DC / 4];
 #pragma unroll
   for (int c = 0; c < DC / 4; ++c) inf[c] = 0;
-  auto mend = [&](int k0, int b) __attribute__((always_inline)) {
-    char* vl = vbuf + b * NW * VB;
+  auto mend = [&](int k0) __attribute__((always_inline)) {
+    char* vl = vbuf;
     bool odd = false, seen = false;
 #pragma nounroll
     for (int p = 0; p < 2 * KS; ++p) {
@@ -998,15 +1051,23 @@ __global__ __launch_bounds__(256) void paged_few_kernel(const PagedArgs a) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   };
 
-  v8 ka[2][KS], kn[2][KS];
-  auto work = [&](int i, int b, v8 (&kf)[2][KS]) __attribute__((always_inline)) {
+  // A tile: its scores as soon as its keys are there; then the next tile's keys are sent for (`more`), then its values
+  // are waited for; the next tile's follow behind their last use.
+  constexpr int OPS = 2 * KS;  // loads of a tile's keys, and of its values
+  auto work = [&](int i, auto more) __attribute__((always_inline)) {
+    constexpr bool MORE = decltype(more)::value;
     const int k0 = kw + i * KU;
+    wait_loads<OPS>();
     f32x4 s[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) s[t] = Mma16<T>::mma(kf[t][ks], qf[ks], s[t]);
+    }
+    if constexpr (MORE) {
+      place(i + 1);
+      issue_k();
     }
     const bool mask = k0 < it.q.st || k0 + KT - 1 > low;
     if (mask) {
@@ -1038,16 +1099,16 @@ __global__ __launch_bounds__(256) void paged_few_kernel(const PagedArgs a) {
         pt[4 * t + e] = (T)p;
       }
     l = l * alpha + sum;  // this lane's keys; the lanes of a row are added up at the end
-    const unsigned vb = va + b * NW * VB;
-    if (mask) mend(k0, b);
+    wait_loads<MORE ? OPS : 0>();
+    if (mask) mend(k0);
 #pragma unroll
     for (int c4 = 0; c4 < DC; c4 += 4) {
       i16x4 lo[4], hi[4];
       // (a column block's 64 columns are 2 KiB; key group 1 lies KS KiB behind group 0)
-      if (c4 == 0) read_v4<0, KS * 1024>(vb, lo, hi);
-      if (c4 == 4) read_v4<2048, KS * 1024>(vb, lo, hi);
-      if (c4 == 8) read_v4<4096, KS * 1024>(vb, lo, hi);
-      if (c4 == 12) read_v4<6144, KS * 1024>(vb, lo, hi);
+      if (c4 == 0) read_v4<0, KS * 1024>(va, lo, hi);
+      if (c4 == 4) read_v4<2048, KS * 1024>(va, lo, hi);
+      if (c4 == 8) read_v4<4096, KS * 1024>(va, lo, hi);
+      if (c4 == 12) read_v4<6144, KS * 1024>(va, lo, hi);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const i16x8 vv = {lo[c][0], lo[c][1], lo[c][2], lo[c][3], hi[c][0], hi[c][1], hi[c][2], hi[c][3]};
@@ -1055,29 +1116,15 @@ __global__ __launch_bounds__(256) void paged_few_kernel(const PagedArgs a) {
       }
     }
   };
-  // operations of one issue() behind which a wait may stop: the V pieces and K loads of the next tile
-  constexpr int AHEAD = 4 * KS;
-  // (the last tiles apart: in one loop the compiler sees a way around the waits, and would wait for all that is in flight)
-  char* const v1 = vbuf + NW * VB;
-  int i = 0;
-  if (n > 0) issue(0, vbuf, ka);
-  for (; i + 2 < n; i += 2) {
-    issue(i + 1, v1, kn);
-    wait_loads<AHEAD>();
-    work(i, 0, ka);
-    issue(i + 2, vbuf, ka);
-    wait_loads<AHEAD>();
-    work(i + 1, 1, kn);
-  }
-  if (i + 1 < n) {
-    issue(i + 1, v1, kn);
-    wait_loads<AHEAD>();
-    work(i, 0, ka);
-    wait_loads();
-    work(i + 1, 1, kn);
-  } else if (i < n) {
-    wait_loads();
-    work(i, 0, ka);
+  if (n > 0) {
+    place(0);
+    issue_k();
+    issue_v();
+    for (int i = 0; i + 1 < n; ++i) {
+      work(i, std::true_type{});
+      issue_v();
+    }
+    work(n - 1, std::false_type{});
   }
 #pragma unroll
   for (int c = 0; c < DC; ++c)
@@ -1117,7 +1164,7 @@ __global__ __launch_bounds__(256) void paged_few_kernel(const PagedArgs a) {
     if (part) {
       const long slot = (long)blockIdx.x * BM + lr;
       *reinterpret_cast<f32x4*>(a.ws + slot * D + d0) = f32x4{x[0], x[1], x[2], x[3]};
-      if (d0 == 0) *reinterpret_cast<f32x2*>(a.ws + a.ws_ml + slot * 2) = f32x2{M, L};
+      if (d0 == 0) *reinterpret_cast<f32x2*>(a.ml + slot * 2) = f32x2{M, L};
     } else {
       const int rr = row0 + lr, t = fdiv(rr, a.g);
       store_row<T, 4>(a, it.q.q0 + t, it.head * (int)a.g.d + rr - t * (int)a.g.d, d0, x, M, L);
@@ -1125,38 +1172,47 @@ __global__ __launch_bounds__(256) void paged_few_kernel(const PagedArgs a) {
   }
 }
 
-// Joins the chunks of a (tile, head): D / 4 threads a row.
-template <typename T, int D, int BM, int KU>
+// Joins the chunks of a (tile, head), in their order: D / 4 threads a row, ROWS rows a workgroup.
+template <typename T, int D, int BM, int ROWS>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a) {
-  Item it;
-  const int lane = threadIdx.x & 63;
-  if (!find_item<BM, KU, true>(a, blockIdx.x, lane, it)) return;
-  if (it.nch <= 1) return;
-  constexpr int TPR = D / 4;
-  const int R = it.q.n * (int)a.g.d;
-  const int lr = blockIdx.y * (256 / TPR) + threadIdx.x / TPR, r = it.tile * BM + lr;
-  if (lr >= BM || r >= R) return;
+  if ((int)blockIdx.x >= a.plan[0]) return;
+  const Record it = *reinterpret_cast<const Record*>(a.plan + PLAN_HEAD + (long)blockIdx.x * RECORD);
+  const int r0 = blockIdx.y * ROWS;
+  if (it.chunks <= 0 || r0 >= it.rows) return;
+  if (it.first + (long)(it.chunks - 1) * it.step >= a.items) return;  // only where q_start descends
+  constexpr int TPR = D / 4, RPB = 256 / TPR, AT = 8;  // chunks on their way at once
   const int d0 = (threadIdx.x % TPR) * 4;
-  const int end = min(tile_end(a, it, BM), (it.u0 + it.units) * KU);
-  const int left = end - it.u0 * KU;
-  const int n = left > 0 ? ((left + KU - 1) / KU + it.cs - 1) / it.cs : 1;  // chunks that wrote
-  if (it.first + (long)(n - 1) * it.step >= a.items) return;  // only where q_start descends
-  const float* ml = a.ws + a.ws_ml;
-  const long s0 = (long)it.first * BM + lr, ds = (long)it.step * BM;
-  float M = NONE;
-  for (int c = 0; c < n; ++c) M = fmaxf(M, ml[(s0 + c * ds) * 2]);
-  float x[4] = {0.f, 0.f, 0.f, 0.f}, L = 0.f;
-  for (int c = 0; c < n; ++c) {
-    const long slot = s0 + c * ds;
-    const f32x2 p = *reinterpret_cast<const f32x2*>(ml + slot * 2);
-    const f32x4 y = *reinterpret_cast<const f32x4*>(a.ws + slot * D + d0);
-    const float w = __builtin_amdgcn_exp2f(p[0] - M);
-    L += p[1] * w;
+  const long ds = (long)it.step * BM;
+  for (int lr = r0 + threadIdx.x / TPR; lr < min(r0 + ROWS, it.rows); lr += RPB) {
+    const long s0 = (long)it.first * BM + lr;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    float M = NONE, L = 0.f;
+    for (int c0 = 0; c0 < it.chunks; c0 += AT) {
+      f32x2 p[AT];
+      f32x4 y[AT];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] += y[i] * w;
+      for (int c = 0; c < AT; ++c) {
+        const long slot = s0 + min(c0 + c, it.chunks - 1) * ds;
+        p[c] = *reinterpret_cast<const f32x2*>(a.ml + slot * 2);
+        y[c] = *reinterpret_cast<const f32x4*>(a.ws + slot * D + d0);
+      }
+      float mn = M;
+#pragma unroll
+      for (int c = 0; c < AT; ++c) mn = fmaxf(mn, p[c][0]);
+      const float old = __builtin_amdgcn_exp2f(M - mn);
+      M = mn;
+      L *= old;
+      x *= old;
+#pragma unroll
+      for (int c = 0; c < AT; ++c) {
+        const float w = c0 + c < it.chunks ? __builtin_amdgcn_exp2f(p[c][0] - M) : 0.f;
+        if (c0 + c < it.chunks) L += p[c][1] * w, x += y[c] * w;
+      }
+    }
+    const int r = it.row0 + lr, tok = fdiv(r, a.g);
+    const float y[4] = {x[0], x[1], x[2], x[3]};
+    store_row<T, 4>(a, it.q0 + tok, it.head * (int)a.g.d + r - tok * (int)a.g.d, d0, y, M, L);
   }
-  const int tok = fdiv(r, a.g), hd = it.head * (int)a.g.d + r - tok * (int)a.g.d;
-  store_row<T, 4>(a, it.q.q0 + tok, hd, d0, x, M, L);
 }
 
 // ---------------------------------------------------------------- host
@@ -1164,7 +1220,7 @@ struct Plan {
   int BM, KU;
   long pairs, items;  // upper bounds: (tile, head) pairs and items
   int slots, split;
-  size_t ml_off, bytes;
+  size_t o_off, ml_off, bytes;
 };
 
 int device_cus() {
@@ -1190,21 +1246,24 @@ Plan make_plan(long rows, int S, int Hq, int Hk, int D, long most) {
   p.KU = few ? 128 : 64;
   const long a = rows * g / p.BM + S, b = rows * ((g + p.BM - 1) / p.BM);
   p.pairs = (a < b ? a : b) * Hk;
-  p.slots = device_cus() * (few && D <= 128 ? 2 : 1);
+  p.slots = device_cus() * (few ? few_per_cu(D) : 1);
   const long least = (rows * g + p.BM - 1) / p.BM * Hk;
-  p.split = most > p.KU && least < 8l * p.slots;
-  p.items = p.split ? p.pairs + 4l * p.slots : p.pairs;
-  p.ml_off = p.split ? (size_t)p.items * p.BM * D : 0;
-  p.bytes = p.split ? (p.ml_off + (size_t)p.items * p.BM * 2) * 4 : 0;
+  // Splitting costs the partial results' way through memory and a second launch (4 us): not for keys that one
+  // workgroup works through in about that, and not where there are tiles enough for four rounds.
+  p.split = most > (few ? 1024 : 256) && least < 4l * p.slots;
+  p.items = !p.split ? p.pairs : p.pairs <= p.slots ? p.slots : p.pairs + 4l * p.slots;
+  p.o_off = (size_t)(PLAN_HEAD + p.pairs * RECORD) * 4;  // bytes, a multiple of 16
+  p.ml_off = p.o_off + (size_t)p.items * p.BM * D * 4;
+  p.bytes = p.split ? p.ml_off + (size_t)p.items * p.BM * 2 * 4 : 0;
   return p;
 }
 
-template <typename T, int D, int BM, int KU>
+template <typename T, int D, int BM>
 int join(PagedArgs& a, const Plan& p, hipStream_t st) {
   OSPO_CHECK_LAUNCH();
   if (!p.split) return OSPO_OK;
-  constexpr int RPB = 256 / (D / 4);
-  paged_join_kernel<T, D, BM, KU><<<dim3((unsigned)p.pairs, (BM + RPB - 1) / RPB), 256, 0, st>>>(a);
+  constexpr int ROWS = 1024 / D;  // rows of one pass
+  paged_join_kernel<T, D, BM, ROWS><<<dim3((unsigned)p.pairs, BM / ROWS), 256, 0, st>>>(a);
   OSPO_CHECK_LAUNCH();
   return OSPO_OK;
 }
@@ -1217,14 +1276,15 @@ int launch(PagedArgs& a, const Plan& p, hipStream_t st) {
       paged_few_kernel<T, D, true><<<grid, 256, 0, st>>>(a);
     else
       paged_few_kernel<T, D, false><<<grid, 256, 0, st>>>(a);
-    return join<T, D, 16, 128>(a, p, st);
+    return join<T, D, 16>(a, p, st);
   }
   constexpr int RB = D > 128 ? 1 : 2;
-  if (a.ps.d % 16 == 0)
+  // (16 keys in one page, and near enough to each other for 32-bit byte offsets)
+  if (a.ps.d % 16 == 0 && a.c_ts < (1l << 26))
     paged_many_kernel<T, D, RB, true><<<grid, 256, 0, st>>>(a);
   else
     paged_many_kernel<T, D, RB, false><<<grid, 256, 0, st>>>(a);
-  return join<T, D, 128 * RB, 64>(a, p, st);
+  return join<T, D, 128 * RB>(a, p, st);
 }
 
 bool shapes_ok(int n, int S, int Hq, int Hk, int D, int n_pages, int page_size, int max_pages) {
@@ -1273,8 +1333,8 @@ extern "C" int ospo_paged_attn(const void* q, long q_ts, long q_hs, const void* 
   a.causal = causal;
   a.qvec = aligned16(q) && q_ts % 8 == 0 && q_hs % 8 == 0;
   a.ovec = aligned16(out) && o_ts % 8 == 0 && o_hs % 8 == 0;
-  a.slots = p.slots, a.split = p.split, a.items = p.items;
-  a.ws = (float*)ws, a.ws_ml = (long)p.ml_off;
+  a.slots = p.slots, a.split = p.split, a.items = p.items, a.pairs = p.pairs;
+  a.plan = (int*)ws, a.ws = (float*)((char*)ws + p.o_off), a.ml = (float*)((char*)ws + p.ml_off);
   if (dtype == DT_BF16) {
     switch (head_dim) {
       case 64: return launch<bf16, 64>(a, p, stream);
