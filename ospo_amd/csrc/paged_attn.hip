@@ -379,20 +379,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   int lim[RB];
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
-    const int r = min(row0 + 32 * b + l32, R - 1);
-    const int tok = fdiv(r, a.g), hd = it.head * (int)a.g.d + r - tok * (int)a.g.d;
+    const int tok = fdiv(min(row0 + 32 * b + l32, R - 1), a.g);
     lim[b] = a.causal ? it.q.kv - it.q.n + tok : it.q.kv - 1;
-    const T* p = (const T*)a.q + (long)(it.q.q0 + tok) * a.q_ts + (long)hd * a.q_hs + 8 * hi;
-    if (a.qvec) {
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) qf[b][ks] = *reinterpret_cast<const v8*>(p + 16 * ks);
-    } else {
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) qf[b][ks][i] = p[16 * ks + i];
-    }
   }
+  auto load_q = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      const int r = min(row0 + 32 * b + l32, R - 1);
+      const int tok = fdiv(r, a.g), hd = it.head * (int)a.g.d + r - tok * (int)a.g.d;
+      const T* p = (const T*)a.q + (long)(it.q.q0 + tok) * a.q_ts + (long)hd * a.q_hs + 8 * hi;
+      if (a.qvec) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) qf[b][ks] = *reinterpret_cast<const v8*>(p + 16 * ks);
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) qf[b][ks][i] = p[16 * ks + i];
+      }
+    }
+  };
   // smallest limit of the wave's rows: tiles that end at or before it need no mask
   const int low = a.causal ? it.q.kv - it.q.n + fdiv(min(row0, R - 1), a.g) : it.q.kv - 1;
 
@@ -617,10 +623,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     At a0{};
     place(0, a0);
     fetch(kc, a0, 0, K0);
+    load_q();
     fetch(vc, a0, 1, V0);
     place(min(1, n - 1), ak);
     fetch(kc, ak, 0, K1);
-    wait_loads();
+    wait_loads<2 * NL>();  // K(0)
     sync_lds();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -633,7 +640,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       const float y = fmaxf(mx[0][b], mx[1][b]);
       m[b] = fmaxf(NONE, fmaxf(y, other_half(y)) * a.cs);
     }
-    sync_lds();  // every wave has read K(0): K(2) takes its place
+    wait_loads();  // V(0) and K(1)
+    sync_lds();    // every wave has read K(0): K(2) takes its place
   }
   wait_loads();  // (nothing is in flight: the compiler sees a way around the wait above, and would wait in the loop)
 
@@ -679,7 +687,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
 #pragma unroll
       for (int u = 0; u < 2; ++u) asm volatile("" : "+v"(pt[b][u]));
     __builtin_amdgcn_sched_barrier(0);
-    if (edge(j + 1)) apply_mask(j + 1, H, y);
+    if (j + 1 < n && edge(j + 1)) apply_mask(j + 1, H, y);
     constexpr int SL = 2 * DC, SE = RB * 16 / (SL * RB) > 0 ? 16 / SL : 1;  // slots; sums and maxima of one
     float t[RB];
 #pragma unroll
@@ -755,13 +763,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
 
   settle();
   // Rows through LDS (the tiles' room: 32 rows of D floats a wave, their 16-byte chunks turned by the row), stored 16
-  // bytes a lane.
+  // bytes a lane.  A lane works out its own row's sum and place and hands them to the lanes that store it.
   float* st = reinterpret_cast<float*>(wave == 0 ? K0 : wave == 1 ? K1 : wave == 2 ? V0 : V1);
   auto at = [&](int row, int chunk) __attribute__((always_inline)) { return row * D + ((chunk ^ (row & (D / 4 - 1) & 31)) << 2); };
+  const int lrow = lane / CH, lcol = (lane % CH) * 8;
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
-    const float L = l[b] + other_half(l[b]);
-    const int lrow = lane / CH, lcol = (lane % CH) * 8;
 #pragma unroll
     for (int c = 0; c < DC; ++c)
 #pragma unroll
@@ -769,6 +776,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
         *reinterpret_cast<f32x4*>(st + at(l32, 8 * c + 2 * k + hi)) =
             f32x4{o[b][c][4 * k], o[b][c][4 * k + 1], o[b][c][4 * k + 2], o[b][c][4 * k + 3]};
     if (flushed || anyinf)
+#pragma nounroll
       for (int i = 0; i < DC * 16; ++i) {
         float* e = st + at(l32, 8 * (i >> 4) + 2 * (i >> 2 & 3) + hi) + (i & 3);
         float x = *e;
@@ -780,24 +788,64 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
         }
         *e = x;
       }
+    const float L = l[b] + other_half(l[b]);
+    const int r0 = row0 + 32 * b, left = R - r0;  // rows of this block that there are
+    const long slot = (long)blockIdx.x * BM + (r0 - R0);
+    const int tok = fdiv(min(r0 + l32, R - 1), a.g), hd = it.head * (int)a.g.d + r0 + l32 - tok * (int)a.g.d;
+    const long off = (long)(it.q.q0 + tok) * a.o_ts + (long)hd * a.o_hs;
+    const int off0 = (int)off, off1 = (int)(off >> 32);
+    const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;  // (a row that saw no key: zeros)
+    if (hi == 0 && l32 < left) {
+      if (part)
+        *reinterpret_cast<f32x2*>(a.ml + (slot + l32) * 2) = f32x2{m[b], L};
+      else if (a.lse)
+        a.lse[(long)(it.q.q0 + tok) * a.l_ts + (long)hd * a.l_hs] = L == 0.f ? -INFINITY : (m[b] + __log2f(L)) * LN2;
+    }
     __builtin_amdgcn_wave_barrier();
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma nounroll  // (once an item: what its code takes to fetch is most of its time)
-    for (int i = 0; i < 32 / RPL; ++i) {
-      const int lr = i * RPL + lrow, r = row0 + 32 * b + lr;
-      const float Lr = __shfl(L, lr, 64), Mr = __shfl(m[b], lr, 64);
-      const f32x4 x0 = *reinterpret_cast<const f32x4*>(st + at(lr, lcol / 4));
-      const f32x4 x1 = *reinterpret_cast<const f32x4*>(st + at(lr, lcol / 4 + 1));
-      if (r >= R) continue;
-      if (part) {
-        const long slot = (long)blockIdx.x * BM + (r - R0);
-        *reinterpret_cast<f32x4*>(a.ws + slot * D + lcol) = x0;
-        *reinterpret_cast<f32x4*>(a.ws + slot * D + lcol + 4) = x1;
-        if (lcol == 0) *reinterpret_cast<f32x2*>(a.ml + slot * 2) = f32x2{Mr, Lr};
-      } else {
-        const int tok = fdiv(r, a.g), hd = it.head * (int)a.g.d + r - tok * (int)a.g.d;
-        const float x[8] = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
-        store_row<T, 8>(a, it.q.q0 + tok, hd, lcol, x, Mr, Lr);
+    auto two = [&](int lr, f32x4 (&x)[2]) __attribute__((always_inline)) {
+      x[0] = *reinterpret_cast<const f32x4*>(st + at(lr, lcol / 4));
+      x[1] = *reinterpret_cast<const f32x4*>(st + at(lr, lcol / 4 + 1));
+    };
+    struct alignas(16) Row { T v[8]; };
+    auto done = [&](int lr, T*& to) __attribute__((always_inline)) {
+      f32x4 x[2];
+      two(lr, x);
+      const float f = __shfl(inv, lr, 64);
+      to = (T*)a.o + ((long)__shfl(off1, lr, 64) << 32 | (unsigned)__shfl(off0, lr, 64)) + lcol;
+      Row y;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y.v[e] = (T)(x[e >> 2][e & 3] * f);  // rounded once
+      return y;
+    };
+    if (part) {
+#pragma unroll
+      for (int i = 0; i < 32 / RPL; ++i) {
+        const int lr = i * RPL + lrow;
+        f32x4 x[2];
+        two(lr, x);
+        float* to = a.ws + (slot + lr) * D + lcol;
+        if (lr < left) {
+          *reinterpret_cast<f32x4*>(to) = x[0];
+          *reinterpret_cast<f32x4*>(to + 4) = x[1];
+        }
+      }
+    } else if (a.ovec) {
+#pragma unroll
+      for (int i = 0; i < 32 / RPL; ++i) {
+        const int lr = i * RPL + lrow;
+        T* to;
+        const Row y = done(lr, to);
+        if (lr < left) *reinterpret_cast<Row*>(to) = y;
+      }
+    } else {
+#pragma nounroll
+      for (int i = 0; i < 32 / RPL; ++i) {
+        const int lr = i * RPL + lrow;
+        T* to;
+        const Row y = done(lr, to);
+        if (lr < left)
+          for (int e = 0; e < 8; ++e) to[e] = y.v[e];
       }
     }
     __builtin_amdgcn_wave_barrier();
