@@ -438,7 +438,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     long u;
     long v[2];
   };
-  int pbase = 0, pv = 0, pn = 0, pg[2];
+  int pbase = 0, pn = 0, pg[2];
+  long pv = 0;  // offset of this lane's page
   auto clampp = [&](int p) __attribute__((always_inline)) { return min(max(p, 0), a.n_pages - 1); };
   auto lookup = [&](int k0) __attribute__((always_inline)) {
 #pragma unroll
@@ -450,10 +451,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       const int pi = fdiv(k0 + wrow, a.ps), pc = min(pi, lastp);
       if (pc - pbase >= 64) {  // 64 page numbers sit on the lanes, the next 64 are on their way
         pbase += 64;
-        pv = clampp(pn);
+        pv = clampp(pn) * a.c_ps;
         pn = bt[min(pbase + 64 + lane, lastp)];
       }
-      at.u = (long)lane_of(pv, pc - pbase) * a.c_ps + (long)(k0 + wrow - pi * (int)a.ps.d) * a.c_ts;
+      const unsigned lo = lane_of((int)pv, pc - pbase), up = lane_of((int)(pv >> 32), pc - pbase);
+      at.u = (long)((unsigned long)up << 32 | lo) + (long)(k0 + wrow - pi * (int)a.ps.d) * (int)a.c_ts;
     } else {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -528,7 +530,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   };
   // tiles that some row of the workgroup sees in part; whether one holds values that are not finite
   const int low0 = a.causal ? it.q.kv - it.q.n + fdiv(R0, a.g) : it.q.kv - 1;
-  auto edge = [&](int t) __attribute__((always_inline)) { return kb + t * KU < it.q.st || kb + t * KU + KU - 1 > low0; };
+  const int clear0 = it.q.st > kb ? (it.q.st - kb + KU - 1) / KU : 0, clear1 = low0 >= kb ? (low0 + 1 - kb) / KU : 0;
+  auto edge = [&](int t) __attribute__((always_inline)) { return t < clear0 || t >= clear1; };
   auto look = [&](int t, const char* vl) __attribute__((always_inline)) {
     if (threadIdx.x == 0) found = 0;
     sync_lds();
@@ -581,27 +584,31 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     sync_lds();
   };
   // O taken out of the way when a maximum grew too much: acc = (acc + O) * alpha, O = 0.  In memory, and rare: vector
-  // registers have no room for O, and the matrix unit's own can only be added to.
-  volatile float acc[RB * DC * 16], out[RB * DC * 16];
+  // registers have no room for O, and the matrix unit's own can only be added to.  (Its place in memory is found only
+  // when it is needed: known ahead, its addresses fill the scalar registers of the whole loop.)
+  float acc[RB * DC * 16], out[RB * DC * 16];
   bool flushed = false;
   auto flush = [&]() __attribute__((always_inline)) {
+    int at0 = 0;
+    asm volatile("" : "+v"(at0));
     settle();
 #pragma unroll
     for (int b = 0; b < RB; ++b)
 #pragma unroll
       for (int c = 0; c < DC; ++c)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) out[(b * DC + c) * 16 + r] = o[b][c][r];
+        for (int r = 0; r < 16; ++r) out[at0 + (b * DC + c) * 16 + r] = o[b][c][r];
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
-      const float mn = fmaxf(m[b], fmaxf(mx[0][b], mx[1][b]));
+      const float most = fmaxf(mx[0][b], mx[1][b]);  // of this lane's keys
+      const float mn = fmaxf(m[b], fmaxf(most, other_half(most)) * a.cs);
       const float alpha = __builtin_amdgcn_exp2f(m[b] - mn);
       m[b] = mn;
       l[b] *= alpha;
 #pragma nounroll
       for (int i = 0; i < DC * 16; ++i) {
-        const int e = b * DC * 16 + i;
+        const int e = at0 + b * DC * 16 + i;
         const float old = flushed ? acc[e] : 0.f;
         acc[e] = (old + out[e]) * alpha;
       }
@@ -615,7 +622,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   if (n > 0) {
     if constexpr (P16) {
       pbase = min(fdiv(kb + wrow, a.ps), lastp);
-      pv = clampp(bt[min(pbase + lane, lastp)]);
+      pv = clampp(bt[min(pbase + lane, lastp)]) * a.c_ps;
       pn = bt[min(pbase + 64 + lane, lastp)];
     } else {
       lookup(kb);
@@ -724,6 +731,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     // V(j + 1) lies where K(j + 1) did and takes the place of V(j - 1); K(j + 2) that of K(j)
     // (behind the last tile: the last again), a piece every other slot of the first half, as a row of them would hold
     // up the wave
+    v8 kf[PF + 1];
+#pragma unroll
+    for (int ks = 0; ks < PF; ++ks) kf[ks] = kfrag(k1, 0, ks);
     av = ak;
     place(min(j + 2, n - 1), ak);
     auto ahead = [&](int p) __attribute__((always_inline)) {
@@ -734,21 +744,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     };
     auto none = [](int) {};
     // raise the maxima where they grew too much
-    bool grow = false;
+    float rise = fmaf(fmaxf(mx[0][0], mx[1][0]), a.cs, -m[0]);
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) mx[h][b] = fmaxf(mx[h][b], other_half(mx[h][b])) * a.cs;
-      grow = grow || fmaxf(mx[0][b], mx[1][b]) > m[b] + F::GROW;
-    }
-    if (__ballot(grow)) flush();
+    for (int b = 1; b < RB; ++b) rise = fmaxf(rise, fmaf(fmaxf(mx[0][b], mx[1][b]), a.cs, -m[b]));
+    if (__ballot(rise > F::GROW)) flush();
     if (edge(j)) {
       const int odd = look(j, v0);
       if (odd) mend(j, v0, odd & 2);
     }
-    v8 kf[PF + 1];
-#pragma unroll
-    for (int ks = 0; ks < PF; ++ks) kf[ks] = kfrag(k1, 0, ks);
     half(j, H0{}, k1, v0, x[0], y[0], kf, ahead);
     half(j, H1{}, k1, v0, x[1], y[1], kf, none);
     wait_loads();
@@ -1328,7 +1331,7 @@ int launch(PagedArgs& a, const Plan& p, hipStream_t st) {
   }
   constexpr int RB = D > 128 ? 1 : 2;
   // (16 keys in one page, and near enough to each other for 32-bit byte offsets)
-  if (a.ps.d % 16 == 0 && a.c_ts < (1l << 26))
+  if (a.ps.d % 16 == 0 && a.c_ts >= 0 && a.c_ts < (1l << 26))
     paged_many_kernel<T, D, RB, true><<<grid, 256, 0, st>>>(a);
   else
     paged_many_kernel<T, D, RB, false><<<grid, 256, 0, st>>>(a);
