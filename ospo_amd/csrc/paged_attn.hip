@@ -350,10 +350,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   using F = Frag<T>;
   using v8 = typename F::v8;
   constexpr int NW = 4, BM = 32 * RB * NW, KU = 64;
-  constexpr int ROWB = D * 2, CH = D / 8, TILE = KU * ROWB;
+  constexpr int ROWB = D * 2, TILE = KU * ROWB;
   constexpr int KS = D / 16, DC = D / 32;
   constexpr int NL = D / 32;    // column blocks: LDS-DMA pieces of a wave's 16 keys
-  constexpr int RPL = 64 / CH;  // rows of a 1-KiB store
   // objects of their own, so that the compiler sees that a read of one does not wait for what is on its way to another
   __shared__ __attribute__((aligned(1024))) char K0[TILE], K1[TILE], V0[TILE], V1[TILE];
   __shared__ int inf[NW][RB * DC][64];  // where a sum is +infinity (bit r) and -infinity (bit 16 + r), see mend
@@ -765,94 +764,70 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
   if (j < n) step(j, K0, K1, V0, V1, s[0], s[1]);
 
   settle();
-  // Rows through LDS (the tiles' room: 32 rows of D floats a wave, their 16-byte chunks turned by the row), stored 16
-  // bytes a lane.  A lane works out its own row's sum and place and hands them to the lanes that store it.
-  float* st = reinterpret_cast<float*>(wave == 0 ? K0 : wave == 1 ? K1 : wave == 2 ? V0 : V1);
-  auto at = [&](int row, int chunk) __attribute__((always_inline)) { return row * D + ((chunk ^ (row & (D / 4 - 1) & 31)) << 2); };
-  const int lrow = lane / CH, lcol = (lane % CH) * 8;
+  // A lane stores its own row: 8 values at a time, after an exchange with the lane that holds the other half of its keys'
+  // columns.  (32 bytes of 32 rows a store, which L2 puts together: through LDS, in whole rows, an item took 2 us more.)
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
+    const float L = l[b] + other_half(l[b]);
+    const int r = row0 + 32 * b + l32, tok = fdiv(min(r, R - 1), a.g), hd = it.head * (int)a.g.d + r - tok * (int)a.g.d;
+    float x[DC][16];
 #pragma unroll
     for (int c = 0; c < DC; ++c)
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        *reinterpret_cast<f32x4*>(st + at(l32, 8 * c + 2 * k + hi)) =
-            f32x4{o[b][c][4 * k], o[b][c][4 * k + 1], o[b][c][4 * k + 2], o[b][c][4 * k + 3]};
-    if (flushed || anyinf)
-#pragma nounroll
-      for (int i = 0; i < DC * 16; ++i) {
-        float* e = st + at(l32, 8 * (i >> 4) + 2 * (i >> 2 & 3) + hi) + (i & 3);
-        float x = *e;
-        if (flushed) x += acc[b * DC * 16 + i];
-        if (anyinf) {
-          const int bits = inf[wave][(i >> 4) * RB + b][lane] >> (i & 15);
-          if (bits & 1) x += INFINITY;
-          if (bits & 65536) x -= INFINITY;
-        }
-        *e = x;
-      }
-    const float L = l[b] + other_half(l[b]);
-    const int r0 = row0 + 32 * b, left = R - r0;  // rows of this block that there are
-    const long slot = (long)blockIdx.x * BM + (r0 - R0);
-    const int tok = fdiv(min(r0 + l32, R - 1), a.g), hd = it.head * (int)a.g.d + r0 + l32 - tok * (int)a.g.d;
-    const long off = (long)(it.q.q0 + tok) * a.o_ts + (long)hd * a.o_hs;
-    const int off0 = (int)off, off1 = (int)(off >> 32);
-    const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;  // (a row that saw no key: zeros)
-    if (hi == 0 && l32 < left) {
-      if (part)
-        *reinterpret_cast<f32x2*>(a.ml + (slot + l32) * 2) = f32x2{m[b], L};
-      else if (a.lse)
-        a.lse[(long)(it.q.q0 + tok) * a.l_ts + (long)hd * a.l_hs] = L == 0.f ? -INFINITY : (m[b] + __log2f(L)) * LN2;
-    }
-    __builtin_amdgcn_wave_barrier();
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    auto two = [&](int lr, f32x4 (&x)[2]) __attribute__((always_inline)) {
-      x[0] = *reinterpret_cast<const f32x4*>(st + at(lr, lcol / 4));
-      x[1] = *reinterpret_cast<const f32x4*>(st + at(lr, lcol / 4 + 1));
-    };
-    struct alignas(16) Row { T v[8]; };
-    auto done = [&](int lr, T*& to) __attribute__((always_inline)) {
-      f32x4 x[2];
-      two(lr, x);
-      const float f = __shfl(inv, lr, 64);
-      to = (T*)a.o + ((long)__shfl(off1, lr, 64) << 32 | (unsigned)__shfl(off0, lr, 64)) + lcol;
-      Row y;
+      for (int i = 0; i < 16; ++i) x[c][i] = o[b][c][i];
+    if (flushed || anyinf) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y.v[e] = (T)(x[e >> 2][e & 3] * f);  // rounded once
-      return y;
-    };
+      for (int c = 0; c < DC; ++c) {
+        const int bits = anyinf ? inf[wave][c * RB + b][lane] : 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if (flushed) x[c][i] += acc[(b * DC + c) * 16 + i];
+          if (bits >> i & 1) x[c][i] += INFINITY;
+          if (bits >> i & 65536) x[c][i] -= INFINITY;
+        }
+      }
+    }
     if (part) {
+      const long slot = (long)blockIdx.x * BM + (r - R0);
+      if (r < R) {
+        if (hi == 0) *reinterpret_cast<f32x2*>(a.ml + slot * 2) = f32x2{m[b], L};
+        float* to = a.ws + slot * D + 4 * hi;
 #pragma unroll
-      for (int i = 0; i < 32 / RPL; ++i) {
-        const int lr = i * RPL + lrow;
-        f32x4 x[2];
-        two(lr, x);
-        float* to = a.ws + (slot + lr) * D + lcol;
-        if (lr < left) {
-          *reinterpret_cast<f32x4*>(to) = x[0];
-          *reinterpret_cast<f32x4*>(to + 4) = x[1];
-        }
-      }
-    } else if (a.ovec) {
+        for (int c = 0; c < DC; ++c)
 #pragma unroll
-      for (int i = 0; i < 32 / RPL; ++i) {
-        const int lr = i * RPL + lrow;
-        T* to;
-        const Row y = done(lr, to);
-        if (lr < left) *reinterpret_cast<Row*>(to) = y;
+          for (int k = 0; k < 4; ++k)
+            *reinterpret_cast<f32x4*>(to + 32 * c + 8 * k) = f32x4{x[c][4 * k], x[c][4 * k + 1], x[c][4 * k + 2], x[c][4 * k + 3]};
       }
-    } else {
-#pragma nounroll
-      for (int i = 0; i < 32 / RPL; ++i) {
-        const int lr = i * RPL + lrow;
-        T* to;
-        const Row y = done(lr, to);
-        if (lr < left)
-          for (int e = 0; e < 8; ++e) to[e] = y.v[e];
-      }
+      continue;
     }
-    __builtin_amdgcn_wave_barrier();
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    const float inv = L > 0.f ? 1.f / L : L == 0.f ? 0.f : L;  // (a row that saw no key: zeros)
+    if (a.lse && hi == 0 && r < R)
+      a.lse[(long)(it.q.q0 + tok) * a.l_ts + (long)hd * a.l_hs] = L == 0.f ? -INFINITY : (m[b] + __log2f(L)) * LN2;
+    T* to = (T*)a.o + (long)(it.q.q0 + tok) * a.o_ts + (long)hd * a.o_hs + 8 * hi;
+#pragma unroll
+    for (int c = 0; c < DC; ++c)
+#pragma unroll
+      for (int k = 0; k < 4; k += 2) {  // columns 32 c + 8 (k + hi) ..
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+        t4 y[2];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          y[0][e] = (T)(x[c][4 * k + e] * inv), y[1][e] = (T)(x[c][4 * k + 4 + e] * inv);  // rounded once
+        const u32x2 lo = __builtin_bit_cast(u32x2, y[0]), up = __builtin_bit_cast(u32x2, y[1]);
+        const auto s0 = __builtin_amdgcn_permlane32_swap(lo[0], up[0], false, false);
+        const auto s1 = __builtin_amdgcn_permlane32_swap(lo[1], up[1], false, false);
+        const u32x4 w = {s0[0], s1[0], s0[1], s1[1]};
+        if (r >= R) continue;
+        if (a.ovec)
+          *reinterpret_cast<u32x4*>(to + 32 * c + 8 * k) = w;
+        else
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const unsigned short u = (unsigned short)(w[e >> 1] >> (16 * (e & 1)));
+            to[32 * c + 8 * k + e] = __builtin_bit_cast(T, u);
+          }
+      }
   }
 }
 
