@@ -185,7 +185,8 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int id, int lane, 
     before += lane_of(upto, 63);
     pairs += lane_of(pupto, 63);
   }
-  if (id == 0 && a.split && threadIdx.x == 0) a.plan[0] = pairs;
+  // (more than the launches' bounds only where q_start descends: nothing is joined then)
+  if (id == 0 && a.split && threadIdx.x == 0) a.plan[0] = before <= a.items && pairs <= a.pairs ? pairs : 0;
   return got;
 }
 // one past the last key that any row of the tile sees
@@ -1205,7 +1206,6 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a) {
   const Record it = *reinterpret_cast<const Record*>(a.plan + PLAN_HEAD + (long)blockIdx.x * RECORD);
   const int r0 = blockIdx.y * ROWS;
   if (it.chunks <= 0 || r0 >= it.rows) return;
-  if (it.first + (long)(it.chunks - 1) * it.step >= a.items) return;  // only where q_start descends
   constexpr int TPR = D / 4, RPB = 256 / TPR, AT = 8;  // chunks on their way at once
   const int d0 = (threadIdx.x % TPR) * 4;
   const long ds = (long)it.step * BM;

@@ -268,6 +268,58 @@ def test_paged_attn_later_values_do_not_reach_earlier_rows(value, new, total, hk
     assert bool(got[row:][keep].isfinite().all())
 
 
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("new,at", [(70, 10), (70, 300), (2, 300)])
+@pytest.mark.parametrize("d,dtype", [(64, HF), (128, BF), (256, BF)])
+def test_paged_attn_values_that_are_not_finite(value, new, at, d, dtype):
+    """At a key that every row sees, in the first tile and in the middle: its column of its head, and nothing else."""
+    s = R.build([new], [500], hq=8, hk=2, d=d, page=16, dtype=dtype, seed=13, device=DEV)
+    args = (s["q"], s["kc"], s["vc"], s["table"], s["q_start"], s["kv_len"], d ** -0.5)
+    clean = ops().paged_attn(*args)
+    s["vc"][int(s["table"][0, at // 16]), 1, at % 16, d - 3] = value
+    got = ops().paged_attn(*args)
+    hit = got[:, 4:, d - 3].float()
+    assert bool((hit.isnan() if math.isnan(value) else hit == value).all())
+    got[:, 4:, d - 3] = clean[:, 4:, d - 3]
+    assert torch.allclose(got.float(), clean.float(), rtol=2.0 ** -7, atol=2.0 ** -9)
+
+
+@pytest.mark.parametrize("new,total", [([130], [700]), ([1, 1, 1], [700, 64, 129]), ([70, 1], [65, 3000])])
+@pytest.mark.parametrize("d,dtype", [(64, HF), (128, BF), (256, BF), (128, HF)])
+@pytest.mark.parametrize("down", [False, True])
+def test_paged_attn_scores_that_grow(new, total, d, dtype, down):
+    """Keys that lengthen (or shorten) along the sequence: maxima rise by many powers of two from tile to tile, and
+    what was summed before has to follow."""
+    s = R.build(new, total, hq=8, hk=2, d=d, page=16, dtype=dtype, seed=12, device=DEV)
+    for b, t in enumerate(total):
+        for i in range(-(-t // 16)):
+            pos = torch.arange(16, device=DEV) + 16 * i
+            f = 1 + ((t - pos).clamp(min=0) if down else pos).float() / 8
+            page = int(s["table"][b, i])
+            s["kc"][page] = (s["kc"][page].float() * f.clamp(max=90.0)[None, :, None]).to(dtype)
+    check(s, d ** -0.5)
+
+
+def test_paged_attn_many_sequences():
+    """More sequences than a wave has lanes, of all lengths, some cut into chunks: single tokens, and chunks beside
+    them; rows of none between."""
+    total = [1 + (37 * i * i) % 700 for i in range(150)]
+    total[3], total[70], total[149] = 9000, 5000, 3000
+    for new in ([1] * 150, [0 if i % 7 == 0 else min(total[i], 1 + 40 * (i % 3 == 0)) for i in range(150)]):
+        s = R.build(new, total, hq=4, hk=1, d=64, page=16, dtype=BF, seed=14, device=DEV, lead=2, tail=3)
+        check(s, 0.125)
+
+
+def test_paged_attn_nothing_to_do():
+    s = R.build([1], [40], hq=4, hk=2, d=64, page=16, dtype=BF, seed=1, device=DEV)
+    none = ops().paged_attn(s["q"][:0], s["kc"], s["vc"], s["table"], torch.zeros(2, dtype=torch.int32, device=DEV),
+                            s["kv_len"], 0.1)
+    assert none.shape == (0, 4, 64)
+    out = torch.full((1, 4, 64), 3.0, device=DEV).to(BF)
+    ops().paged_attn(s["q"], s["kc"], s["vc"], s["table"][:0], s["q_start"][:1], s["kv_len"][:0], 0.1, out=out)
+    assert bool((out == 3).all())
+
+
 @pytest.mark.parametrize("new,total", [([1, 1], [700, 90]), ([130], [900])])
 @pytest.mark.parametrize("d", [64, 128])
 def test_paged_attn_strides_streams_and_offsets(new, total, d):
