@@ -1,5 +1,5 @@
-"""Which hipBLASLt kernel torch.matmul picks for the step's NT GEMM shapes (for study of its
-schedule with llvm-objdump), and its time per launch.  rocprofv3 --kernel-trace --stats -- python tools/blaslt_probe.py"""
+"""Which hipBLASLt kernel torch.matmul picks for the step's NT GEMM shapes, and its time per launch.
+rocprofv3 --kernel-trace --stats -- python tools/blaslt_probe.py"""
 import torch
 
 torch.backends.cuda.matmul.allow_tf32 = False
