@@ -967,6 +967,12 @@ def _heads(t: torch.Tensor, name: str, dtype, n: int, d: int) -> tuple:
     return sh[1], st[0], st[1]
 
 
+def _written(t: torch.Tensor, name: str) -> None:
+    """Refuses a tensor to write to whose elements share memory (an expanded one)."""
+    if 0 in t.stride() and any(m > 1 and st == 0 for m, st in zip(t.shape, t.stride())):
+        raise ValueError(f"{name}: elements of an expanded tensor share memory: strides {t.stride()}")
+
+
 def _ints(t: torch.Tensor, name: str, shape: tuple) -> None:
     if t.dtype != _I32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name}: expected a contiguous int32 tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
@@ -1029,6 +1035,9 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, 
         qo, ko = out
         if qo.shape != q.shape or (ko is None) != (k is None) or (k is not None and ko.shape != k.shape):
             raise ValueError("rotary: out has other shapes than q and k")
+        _written(qo, "out[0]")
+        if ko is not None:
+            _written(ko, "out[1]")
     _, qo0, qo1 = _heads(qo, "out[0]", dt, n, d)
     if k is None:
         hk = k0 = k1 = ko0 = ko1 = 0
@@ -1082,6 +1091,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     hv, v0, v1 = _heads(v, "v", dt, n, d)
     n_pages, heads, page, n_seqs, max_pages, st = _paged("paged_append", k_cache, v_cache, block_table, q_start, kv_len,
                                                          dt, d)
+    _written(k_cache, "k_cache")
     if hv != hk or heads != hk:
         raise ValueError(f"paged_append: {hk} heads in k, {hv} in v, {heads} in the cache")
     if not 1 <= d <= 256:
@@ -1101,6 +1111,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
             q_out = q.new_empty(q.shape)
         elif q_out.shape != q.shape:
             raise ValueError("paged_append: q_out has another shape than q")
+        else:
+            _written(q_out, "q_out")
         _, qo0, qo1 = _heads(q_out, "q_out", dt, n, d)
         qp, qop = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
@@ -1152,12 +1164,15 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
         out = q.new_empty(q.shape)
     elif out.shape != q.shape:
         raise ValueError("paged_attn: out has another shape than q")
+    else:
+        _written(out, "out")
     _, o0, o1 = _heads(out, "out", dt, n, d)
     l0 = l1 = 0
     lp = None
     if lse is not None:
         if lse.dtype != _F32 or lse.shape != (n, hq):
             raise ValueError(f"paged_attn: lse is fp32 [{n}, {hq}], got {lse.dtype} {tuple(lse.shape)}")
+        _written(lse, "lse")
         l0, l1 = lse.stride()
         lp = lse.data_ptr()
     index = _place("paged_attn", q, k_cache, v_cache, block_table, q_start, kv_len, out, start, lse)

@@ -203,6 +203,28 @@ def test_c_attn_refusals(kw, rc):
     assert c_attn(**kw) == rc
 
 
+def test_outputs_whose_elements_share_memory_are_refused():
+    wide = torch.zeros(3, 1, 64, dtype=BF).expand(3, 4, 64)
+    rows = torch.zeros(1, 2, 64, dtype=BF).expand(3, 2, 64)
+    pages = torch.zeros(1, 2, 16, 64, dtype=BF).expand(5, 2, 16, 64)
+    with pytest.raises(ValueError, match="share memory"):
+        _rot(out=(wide, torch.zeros(3, 2, 64, dtype=BF)))
+    with pytest.raises(ValueError, match="share memory"):
+        _rot(out=(torch.zeros(3, 4, 64, dtype=BF), rows))
+    for kw in (dict(q_out=wide), dict(kc=pages, vc=pages)):
+        a = _cache(**kw)
+        with pytest.raises(ValueError, match="share memory"):
+            ops.paged_append(a["k"], a["v"], a["kc"], a["vc"], a["table"], a["q_start"], a["kv_len"], q=a["q"],
+                             q_out=a["q_out"])
+    for kw in (dict(out=wide), dict(lse=torch.zeros(3, 1).expand(3, 4))):
+        a = _cache(**kw)
+        with pytest.raises(ValueError, match="share memory"):
+            ops.paged_attn(a["q"], a["kc"], a["vc"], a["table"], a["q_start"], a["kv_len"], 0.1, out=a["out"], lse=a["lse"])
+    # inputs may be expanded
+    with pytest.raises(ValueError, match="device tensors"):
+        _rot(q=wide, k=rows)
+
+
 def test_division_by_a_multiply_is_exact():
     """The kernels' n / d (paged.h, make_fdiv and fdiv) for the divisors and dividends where it could go wrong."""
     for d in list(range(1, 300)) + [511, 512, 513, 1000, 4095, 4096, 65535, 65537, 2 ** 30 - 1, 2 ** 30, 2 ** 31 - 1]:
