@@ -343,10 +343,11 @@ constexpr int pitch_of(int D) { return D + 4; }  // floats of a staged output ro
 // bf16, 12 in fp16): probabilities then reach at most 2^GROW, which both types hold with no loss of relative
 // precision, and sums stay in fp32.
 //
-// Measured: whole prompts of 3.5k to 4k tokens, 32 heads over 8 of 128, at 958 TFLOP/s (494 us for four).  A tile of 64
-// keys takes 3600 cycles, 2048 of them products: one wave a SIMD issues 580 instructions a tile, about 5 cycles each.  The
-// start of an item (lengths, page numbers, first keys: three round trips to memory, one behind the other) and its end take
-// 7 us.
+// Measured: whole prompts of 3.5k to 4k tokens, 32 heads over 8 of 128, at 957 TFLOP/s (494 us for four).  A tile of 64
+// keys takes 3600 cycles, 2048 of them products; the matrix unit is busy for 54 % of all cycles.  32 instructions less a
+// tile (of 580) change nothing, no exponentials at all would gain 7 %, fragments read 2 or 4 slots ahead the same time.
+// The start of an item (lengths, page numbers, first keys: three round trips to memory, one behind the other) and its end
+// take 7 us.
 //
 // LDS images: blocks of 16 keys x 32 columns, 1 KiB each, [16-byte chunk q of the columns][key, for V key ^ 4 q]: every
 // fragment is one address and a constant, and the reads of K (16 keys of a chunk) and the transposed reads of V (4
