@@ -839,7 +839,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
 }
 
 // ---------------------------------------------------------------- few rows
-// Up to 16 rows for each sequence and key/value head (single tokens): the keys' bytes bound it.  Four waves share out
+// Few rows for each sequence and key/value head (single tokens), in tiles of 16: the keys' bytes bound it.  Four waves share out
 // the key tiles (32 keys each); a wave streams on its own, with no barrier until the end.  A tile's keys come into
 // registers (as they lie in memory they are the A operand of S^T = K Q^T), its values into LDS, from where the
 // transposed reads of O^T += V^T P^T take them.  16 x 16 x 32 products: a 32-row form would spend twice the
@@ -1267,13 +1267,14 @@ int device_cus() {
   return cus[dev];
 }
 
-// At most 16 rows for each sequence and key/value head on average (single tokens of groups up to 16): the kernel for
-// few rows.  Otherwise the one for many (256-row tiles; 128 with 256-wide heads, whose O fills the registers at 32 rows
-// a wave).
+// At most 32 rows for each sequence and key/value head on average: the kernel for few rows.  Otherwise the one for many
+// (256-row tiles; 128 with 256-wide heads, whose O fills the registers at 32 rows a wave).  32 heads over 8 of 128, few
+// against many: 8 sequences of 4000 keys with 16, 32, 64 rows 31 / 38, 42 / 38, 67 / 40 us; 64 of 1000 keys 48 / 92,
+// 65 / 98, 122 / 109 us.
 Plan make_plan(long rows, int S, int Hq, int Hk, int D, long most) {
   Plan p;
   const long g = Hq / Hk;
-  const bool few = rows * g <= 16l * S;
+  const bool few = rows * g <= 32l * S;
   p.BM = few ? 16 : D > 128 ? 128 : 256;
   p.KU = few ? 128 : 64;
   const long a = rows * g / p.BM + S, b = rows * ((g + p.BM - 1) / p.BM);

@@ -7,6 +7,8 @@
 //
 // Memory bound: every element is read once and written once.  A thread owns one unit (W elements and their
 // partners) of one token and walks the heads, so a token's cos / sin are read once per unit and not per head.
+// Measured: 32 + 32 heads of 128 for 4800 tokens (158 MB) in 26.9 us, 5.9 TB/s; the append of 8192 tokens with 32 + 8 heads
+// of 128 (206 MB) in 41.9 us, 4.9 TB/s.  A copy of 4 GiB reaches 4.8 TB/s; these sizes sit partly in the Infinity Cache.
 #include "paged.h"
 
 namespace {
@@ -247,7 +249,8 @@ int launch(RotArgs& a, int W, int il, int dtype, hipStream_t st) {
 }
 
 // Widest load (elements) that every row, head and unit of the call allows: a power of two up to 16 bytes that
-// divides the sizes and strides and to which the pointers are aligned.
+// divides the sizes and strides and to which the pointers are aligned.  (The append of 8192 tokens at 16, 8 and 2 bytes
+// a load: 45, 49 and 83 us.)
 struct Width {
   int es;
   int w;

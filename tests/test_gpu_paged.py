@@ -268,6 +268,19 @@ def test_paged_attn_later_values_do_not_reach_earlier_rows(value, new, total, hk
     assert bool(got[row:][keep].isfinite().all())
 
 
+@pytest.mark.parametrize("new,total,page,hq,hk", [
+    ([8, 8], [300, 40], 16, 8, 2),
+    ([20, 1, 1, 1], [900, 64, 5, 33], 24, 8, 2),
+    ([9, 3], [5000, 3], 64, 28, 4),
+    ([33, 31], [1500, 31], 16, 4, 4),  # on both sides of the rule
+    ([32], [2000], 8, 2, 2),
+    ([33], [2000], 8, 2, 2)])
+@pytest.mark.parametrize("d,dtype", [(64, HF), (128, BF), (256, BF)])
+def test_paged_attn_a_few_tiles_of_rows(new, total, page, hq, hk, d, dtype):
+    s = R.build(new, total, hq=hq, hk=hk, d=d, page=page, dtype=dtype, seed=15, device=DEV, tail=1, fill=math.nan)
+    check(s, d ** -0.5)
+
+
 @pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
 @pytest.mark.parametrize("new,at", [(70, 10), (70, 300), (2, 300)])
 @pytest.mark.parametrize("d,dtype", [(64, HF), (128, BF), (256, BF)])
