@@ -1281,9 +1281,13 @@ Plan make_plan(long rows, int S, int Hq, int Hk, int D, long most) {
   p.pairs = (a < b ? a : b) * Hk;
   p.slots = device_cus() * (few ? few_per_cu(D) : 1);
   const long least = (rows * g + p.BM - 1) / p.BM * Hk;
-  // Splitting costs the partial results' way through memory and a second launch (4 us): not for keys that one
-  // workgroup works through in about that, and not where there are tiles enough for four rounds.
-  p.split = most > (few ? 1024 : 256) && least < 4l * p.slots;
+  // Splitting costs the partial results' way through memory and a second launch.  It pays from more keys on the less room
+  // the tiles leave for chunks, and not where there are tiles enough for four rounds.  Not split against split: one
+  // token, 8 key/value heads of 128, 400, 700, 1000, 4000 keys 12 / 16, 16 / 16, 20 / 16, 60 / 15 us; 64 tokens over 200,
+  // 1000, 4000: 20 / 18, 37 / 21, 105 / 28; four chunks of 256 tokens (half of the slots) over 200, 1000, 1500, 4000:
+  // 26 / 35, 42 / 45, 55 / 52, 112 / 86.
+  const long bar = few ? 640 + 384 * p.pairs / p.slots : 256 + 2048 * p.pairs / p.slots;
+  p.split = most > bar && least < 4l * p.slots;
   p.items = !p.split ? p.pairs : p.pairs <= p.slots ? p.slots : p.pairs + 4l * p.slots;
   p.o_off = (size_t)(PLAN_HEAD + p.pairs * RECORD) * 4;  // bytes, a multiple of 16
   p.ml_off = p.o_off + (size_t)p.items * p.BM * D * 4;
