@@ -1285,7 +1285,7 @@ Plan make_plan(long rows, int S, int Hq, int Hk, int D, long most) {
   // the tiles leave for chunks, and not where there are tiles enough for four rounds.  Not split against split: one
   // token, 8 key/value heads of 128, 400, 700, 1000, 4000 keys 12 / 16, 16 / 16, 20 / 16, 60 / 15 us; 64 tokens over 200,
   // 1000, 4000: 20 / 18, 37 / 21, 105 / 28; four chunks of 256 tokens (half of the slots) over 200, 1000, 1500, 4000:
-  // 26 / 35, 42 / 45, 55 / 52, 112 / 86.
+  // 26 / 35, 42 / 45, 55 / 52, 112 / 86; four of 512 (all slots) over 0, 512, 1000: 26 / 33, 41 / 47, 56 / 62.
   const long bar = few ? 640 + 384 * p.pairs / p.slots : 256 + 2048 * p.pairs / p.slots;
   p.split = most > bar && least < 4l * p.slots;
   p.items = !p.split ? p.pairs : p.pairs <= p.slots ? p.slots : p.pairs + 4l * p.slots;
