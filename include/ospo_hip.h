@@ -560,7 +560,7 @@ int ospo_decode_attn_o(const void* q, int ldq, const void* k_cache, const void* 
  * ospo_paged_attn: out[r][h] = softmax(scale q[r][h] . K) V over the keys max(0, start[s]) .. position of r
  *   (causal = 1) or .. kv_len[s] - 1 (causal = 0); start NULL: 0.  Query head h reads key/value head
  *   h / (n_q_heads / n_kv_heads).  fp32 scores, softmax statistics and sums; probabilities enter the second product
- *   in the cache's type.  lse (optional, fp32 by l_ts, l_hs): natural log of the sum of exponentials.  A row that
+ *   in the cache's type (fp16: to its 11 bits down to 2^-22 of the row's largest, zero below 2^-33).  lse (optional, fp32 by l_ts, l_hs): natural log of the sum of exponentials.  A row that
  *   sees no key: zeros, lse = -inf.  What a row does not see (values of NaN or infinity included) does not change
  *   it.  head_dim 64, 128 or 256; caches 16-byte aligned with strides that are multiples of 8; scale > 0, finite.
  *   ws (16-byte aligned, >= ospo_paged_attn_ws_bytes, contents don't matter): partial results of rows whose keys

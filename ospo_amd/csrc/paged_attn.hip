@@ -217,13 +217,19 @@ __device__ __forceinline__ void note(const PagedArgs& a, const Item& it, int end
 // such a product needs: two states behind the vector unit's last write to an operand, which the block brings along,
 // and settle() before anything but another product reads the accumulators.
 __device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 7" ::: "memory"); }
+//
+// A probability is held as exp2(x - m) in the cache's type, m = the row's largest x less FEW or MANY (few and many rows).
+// bf16 has fp32's exponents and needs no such offset.  fp16's last normal number is 2^-14 and its largest is 65504:
+// from 2^15 at the largest score down, probabilities keep their 11 bits to 2^-29 of the row's largest and end at 2^-40
+// (many rows, which leave a maximum as it is until it grew by 2^7: 2^-22 and 2^-33).  Without an offset they end at 2^-25,
+// and a key that takes a row to itself with a value near zero would leave out what all others add up to.
 template <typename T>
 struct Frag;
 template <>
 struct Frag<bf16> {
   typedef bf16x8 v8;
   static constexpr unsigned EXP = 0x7f80, MAN = 0x007f;
-  static constexpr float GROW = 24.f;
+  static constexpr float GROW = 24.f, FEW = 0.f, MANY = 0.f;
   __device__ static void acc(f32x16& c, const bf16x8& x, const bf16x8& y) {
     asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(x), "v"(y));
   }
@@ -238,7 +244,7 @@ template <>
 struct Frag<f16> {
   typedef f16x8 v8;
   static constexpr unsigned EXP = 0x7c00, MAN = 0x03ff;
-  static constexpr float GROW = 12.f;
+  static constexpr float GROW = 15.f, FEW = 15.f, MANY = 8.f;
   __device__ static void acc(f32x16& c, const f16x8& x, const f16x8& y) {
     asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(c) : "v"(x), "v"(y));
   }
@@ -339,9 +345,9 @@ constexpr int pitch_of(int D) { return D + 4; }  // floats of a staged output ro
 // while O takes tile j, sums of tile j and maxima of tile j + 1 are taken.  (64 keys at a time need more vector
 // registers than there are.)  K(j + 2) and V(j + 1) come by LDS-DMA with the whole tile's time to arrive: one barrier
 // a tile.
-// The running maximum is raised (and O put aside) only when some row's grew by more than GROW powers of two (24 in
-// bf16, 12 in fp16): probabilities then reach at most 2^GROW, which both types hold with no loss of relative
-// precision, and sums stay in fp32.
+// The running maximum is raised (and O scaled) only when a score would reach more than 2^GROW (24 in bf16, 15 in fp16),
+// which both types hold; sums stay in fp32.  (O is scaled where it is: put aside in memory and added up at the end, fp16's
+// chunks of up to 257 tokens over up to 5000 keys, a few of whose rows grow by 2^7, took 42 us instead of 21.)
 //
 // Measured: whole prompts of 3.5k to 4k tokens, 32 heads over 8 of 128, at 957 TFLOP/s (494 us for four).  A tile of 64
 // keys takes 3600 cycles, 2048 of them products; the matrix unit is busy for 54 % of all cycles.  32 instructions less a
@@ -589,39 +595,28 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     }
     sync_lds();
   };
-  // O taken out of the way when a maximum grew too much: acc = (acc + O) * alpha, O = 0.  In memory, and rare: vector
-  // registers have no room for O, and the matrix unit's own can only be added to.  (Its place in memory is found only
-  // when it is needed: known ahead, its addresses fill the scalar registers of the whole loop.)
-  float acc[RB * DC * 16], out[RB * DC * 16];
-  bool flushed = false;
-  auto flush = [&]() __attribute__((always_inline)) {
-    int at0 = 0;
-    asm volatile("" : "+v"(at0));
+  // The maxima raised, O and the sums scaled to them: in the matrix unit's registers, one value at a time (rare; the vector
+  // registers have no room for O).
+  auto raise = [&]() __attribute__((always_inline)) {
     settle();
-#pragma unroll
-    for (int b = 0; b < RB; ++b)
-#pragma unroll
-      for (int c = 0; c < DC; ++c)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) out[at0 + (b * DC + c) * 16 + r] = o[b][c][r];
-    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
       const float most = fmaxf(mx[0][b], mx[1][b]);  // of this lane's keys
-      const float mn = fmaxf(m[b], fmaxf(most, other_half(most)) * a.cs);
+      const float mn = fmaxf(m[b], fmaf(fmaxf(most, other_half(most)), a.cs, -F::MANY));
       const float alpha = __builtin_amdgcn_exp2f(m[b] - mn);
       m[b] = mn;
       l[b] *= alpha;
-#pragma nounroll
-      for (int i = 0; i < DC * 16; ++i) {
-        const int e = at0 + b * DC * 16 + i;
-        const float old = flushed ? acc[e] : 0.f;
-        acc[e] = (old + out[e]) * alpha;
-      }
+#pragma unroll
+      for (int c = 0; c < DC; ++c)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float x = o[b][c][r], t;
+          asm volatile("v_accvgpr_read_b32 %1, %0\n\tv_mul_f32 %1, %1, %2\n\tv_accvgpr_write_b32 %0, %1"
+                       : "+a"(x), "=&v"(t)
+                       : "v"(alpha));
+          o[b][c][r] = x;
+        }
     }
-    clear_o();
-    flushed = true;
-    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0), here and not on the path that goes around
   };
 
   At ak{}, av{};  // of K(j + 1) / V(j + 1) at the start of step j
@@ -651,7 +646,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
       const float y = fmaxf(mx[0][b], mx[1][b]);
-      m[b] = fmaxf(NONE, fmaxf(y, other_half(y)) * a.cs);
+      m[b] = fmaxf(NONE, fmaf(fmaxf(y, other_half(y)), a.cs, -F::MANY));
     }
     wait_loads();  // V(0) and K(1)
     sync_lds();    // every wave has read K(0): K(2) takes its place
@@ -753,7 +748,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     float rise = fmaf(fmaxf(mx[0][0], mx[1][0]), a.cs, -m[0]);
 #pragma unroll
     for (int b = 1; b < RB; ++b) rise = fmaxf(rise, fmaf(fmaxf(mx[0][b], mx[1][b]), a.cs, -m[b]));
-    if (__ballot(rise > F::GROW)) flush();
+    if (__ballot(rise > F::GROW)) raise();
     if (edge(j)) {
       const int odd = look(j, v0);
       if (odd) mend(j, v0, odd & 2);
@@ -782,13 +777,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
     for (int c = 0; c < DC; ++c)
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[c][i] = o[b][c][i];
-    if (flushed || anyinf) {
+    if (anyinf) {
 #pragma unroll
       for (int c = 0; c < DC; ++c) {
-        const int bits = anyinf ? inf[wave][c * RB + b][lane] : 0;
+        const int bits = inf[wave][c * RB + b][lane];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          if (flushed) x[c][i] += acc[(b * DC + c) * 16 + i];
           if (bits >> i & 1) x[c][i] += INFINITY;
           if (bits >> i & 65536) x[c][i] -= INFINITY;
         }
@@ -1118,7 +1112,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_per_cu(
 #pragma unroll
       for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[t][e]);
     mx = max_groups(mx);
-    const float mn = fmaxf(m, mx * a.cs);
+    const float mn = fmaxf(m, fmaf(mx, a.cs, -Frag<T>::FEW));
     const float alpha = __builtin_amdgcn_exp2f(m - mn);
     m = mn;
     float sum = 0.f;
