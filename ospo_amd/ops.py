@@ -1011,15 +1011,54 @@ def _launch(index: int, name: str, *args) -> None:
         _lib.check(name, rc)
 
 
+_recording = torch.is_grad_enabled
+
+
+def _lost_gradient(who: str) -> ValueError:
+    return ValueError(f"{who}: no gradient is recorded through this call: detach its tensors, or call it under "
+                      "torch.no_grad()")
+
+
+class _Rotary(torch.autograd.Function):
+    """Autograd of ``rotary``: it is linear in q and k, and its gradient is the rotation the other way."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, cos, sin, interleaved, backward):
+        ctx.save_for_backward(positions, cos, sin)
+        ctx.interleaved, ctx.turn_back = interleaved, backward
+        ctx.set_materialize_grads(False)
+        return rotary(q, k, positions, (cos, sin), interleaved=interleaved, backward=backward)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        positions, cos, sin = ctx.saved_tensors
+        # (a gradient may come expanded: the last dimension has to be contiguous)
+        grads = [g if g is None or g.stride(2) == 1 else g.contiguous() for g in (dq, dk)]
+        some = [g for g in grads if g is not None]
+        if some:
+            turned = rotary(some[0], some[1] if len(some) > 1 else None, positions, (cos, sin),
+                            interleaved=ctx.interleaved, backward=not ctx.turn_back)
+            grads = [None if g is None else turned[i and len(some) - 1] for i, g in enumerate(grads)]
+        return grads[0], grads[1], None, None, None, None, None
+
+
 def rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, tables: tuple, *,
            interleaved: bool = False, backward: bool = False, out: Optional[tuple] = None) -> tuple:
     """Rotary positions on q [n, q_heads, head_dim] and k [n, kv_heads, head_dim] (or None) of any strides: the first
     rot_dim = 2 * tables[0].shape[1] elements of a head turn by the tables' row of the token's position (int32 [n],
     clamped to the tables), in pairs (i, i + rot_dim / 2), or (2i, 2i + 1) with ``interleaved``; the rest is copied.
-    fp32 arithmetic, rounded once to q's type (bf16, fp16, fp32).  ``backward``: q and k are the gradients of the
-    outputs, the result those of the inputs.  ``out`` (q', k'): where to write, the inputs themselves allowed; new
-    tensors by default.  Returns (q', k')."""
+    fp32 arithmetic, rounded once to q's type (bf16, fp16, fp32).  Gradients of q and k are recorded.  ``backward``: q
+    and k are the gradients of the outputs, the result those of the inputs.  ``out`` (q', k'): where to write, q and k
+    themselves allowed, each in its own place (no gradient is recorded then); new tensors by default.  Returns
+    (q', k')."""
     cos, sin, n_pos, rot = _rot_tables(tables, "rotary")
+    if _recording():
+        if cos.requires_grad or sin.requires_grad:
+            raise _lost_gradient("rotary, to its tables")
+        if q.requires_grad or (k is not None and k.requires_grad):
+            if out is not None:
+                raise _lost_gradient("rotary with out")
+            return _Rotary.apply(q, k, positions, cos, sin, interleaved, backward)
     dt = q.dtype
     code = _CODE.get(dt)
     if q.dim() != 3 or code is None:
@@ -1080,7 +1119,9 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     ``rotary_tables``; None: stored as they are).  Rows q_start[s] .. q_start[s + 1] - 1 are sequence s's newest
     tokens, kv_len[s] its length with them, block_table[s] its pages (all int32, read on the device).  With ``q``
     [n, q_heads, head_dim] its turned copy is returned (``q_out``; may be q itself).  Rows of no sequence are left
-    alone; a row whose position or page does not exist is not stored."""
+    alone; a row whose position or page does not exist is not stored.  Records no gradient."""
+    if _recording() and (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad)):
+        raise _lost_gradient("paged_append")
     dt = k.dtype
     code = _CODE.get(dt)
     if k.dim() != 3 or code is None:
@@ -1140,7 +1181,10 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
     start[s] (default 0) .. its own position, or .. kv_len[s] - 1 with ``causal`` false; query head h reads kv head
     h // (q_heads // kv_heads).  One call takes chunks and single tokens together.  Returns out [n, q_heads,
     head_dim]; lse (fp32 [n, q_heads], optional) gets the natural log of each row's sum of exponentials.  A row that
-    sees nothing is zero, its lse -inf; rows of no sequence are left as they were (in a new ``out``: anything)."""
+    sees nothing is zero, its lse -inf; rows of no sequence are left as they were (in a new ``out``: anything).
+    Records no gradient."""
+    if _recording() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
+        raise _lost_gradient("paged_attn")
     dt = q.dtype
     if q.dim() != 3 or dt not in _PAGED_TYPES:
         raise ValueError(f"paged_attn: expected q [n, heads, head_dim] in bf16 or fp16, got {dt} {tuple(q.shape)}")

@@ -56,3 +56,119 @@ def test_small_probabilities_keep_their_sum(new, total, gap, d, dtype):
         ref = rest.repeat_interleave(hq // hk, 0)
         ok, worst = R.within(out[r], ref, (h + 2 * kv * u + 2.0 ** -17) * ref.abs(), dtype)
         assert ok, (r, worst)
+
+
+# ---------------------------------------------------------------- gradients
+def turn(x, cos, sin, il):
+    """The formula in elementary 64-bit operations that autograd follows."""
+    half = cos.shape[1]
+    c, s = cos.double()[:, None], sin.double()[:, None]
+    a, b = (x[..., 0:2 * half:2], x[..., 1:2 * half:2]) if il else (x[..., :half], x[..., half:2 * half])
+    a, b = a * c - b * s, b * c + a * s
+    y = torch.stack([a, b], -1).flatten(-2) if il else torch.cat([a, b], -1)
+    return torch.cat([y, x[..., 2 * half:]], -1)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("il", [False, True])
+@pytest.mark.parametrize("back", [False, True])
+@pytest.mark.parametrize("hk", [0, 2])
+def test_rotary_records_gradients(dtype, il, back, hk):
+    """Against the formula's gradient: each value is two products and a sum in fp32, rounded once (rotate's bound)."""
+    n, hq, d, rot = 33, 5, 64, 48
+    g = gen(31)
+    q = torch.randn(n, hq, d, generator=g, device=DEV).to(dtype).requires_grad_()
+    k = torch.randn(n, hk, d, generator=g, device=DEV).to(dtype).requires_grad_() if hk else None
+    pos = torch.randint(0, 512, (n,), generator=g, device=DEV).int()
+    tab = ops().rotary_tables(512, rot, 10000.0, DEV)
+    got = ops().rotary(q, k, pos, tab, interleaved=il, backward=back)
+    with torch.no_grad():
+        plain = ops().rotary(q, k, pos, tab, interleaved=il, backward=back)
+    cos, sin = (t[pos.long()] for t in tab)
+    for x, y, p in ((q, got[0], plain[0]), (k, got[1], plain[1])):
+        if x is None:
+            assert y is None
+            continue
+        assert torch.equal(y, p) and y.requires_grad
+        dy = torch.randn(x.shape, generator=g, device=DEV).to(dtype)
+        x64 = x.detach().double().requires_grad_()
+        turn(x64, cos, -sin if back else sin, il).backward(dy.double())
+        (dx,) = torch.autograd.grad(y, x, dy, retain_graph=True)
+        _, tol = R.rotate(dy, torch.atan2(sin.double(), cos.double()), 1.0, il)
+        ok, worst = R.within(dx, x64.grad, tol, dtype)
+        assert ok, worst
+
+
+def test_rotary_gradients_of_one_output_expanded_and_twice():
+    n, d = 9, 32
+    g = gen(32)
+    q, k = (torch.randn(n, h, d, generator=g, device=DEV, requires_grad=True) for h in (4, 2))
+    pos = torch.arange(n, device=DEV).int()
+    tab = ops().rotary_tables(16, d, 10000.0, DEV)
+    qo, ko = ops().rotary(q, k, pos, tab)
+    one = torch.ones(n, 2, d, device=DEV)
+    want = ops().rotary(one, None, pos, tab, backward=True)[0]
+    ko.sum().backward()  # the gradient of a sum comes expanded; q has no part in it
+    assert q.grad is None and torch.equal(k.grad, want)
+    # one of two that wants a gradient; two in one backward pass
+    q2 = q.detach()
+    qo, ko = ops().rotary(q2, k, pos, tab)
+    (dk,) = torch.autograd.grad(ko.sum() + (qo * qo).sum(), k)
+    assert torch.equal(dk, want)
+    # the gradient's gradient: f = sum (R q)^2 w, df/dq = 2 R^T (w R q), its derivative along u is 2 R^T (w R u)
+    w, u = (torch.randn(n, 4, d, generator=g, device=DEV) for _ in range(2))
+    y, _ = ops().rotary(q, None, pos, tab)
+    (dq,) = torch.autograd.grad((y * y * w).sum(), q, create_graph=True)
+    (h,) = torch.autograd.grad((dq * u).sum(), q)
+    with torch.no_grad():
+        ru = ops().rotary(u, None, pos, tab)[0]
+        ref = 2 * ops().rotary(w * ru, None, pos, tab, backward=True)[0]
+    # each of the two rotations and two products rounds its values once: 8 half steps of |w| |u| sums of two
+    assert float((h - ref).abs().max()) <= 8 * 2.0 ** -24 * 2 * 2 * float((w.abs().max() * u.abs().max()) * 2)
+
+
+def test_rotary_gradient_matches_differences_through_autograd():
+    """Along a direction u: the map is linear, so a difference over a step of 1 is exact up to rounding."""
+    n, h, d, rot = 17, 3, 64, 40
+    g = gen(33)
+    x, u, dy = (torch.randn(n, h, d, generator=g, device=DEV) for _ in range(3))
+    pos = torch.arange(n, device=DEV).int()
+    tab = ops().rotary_tables(64, rot, 10000.0, DEV, {"type": "ntk", "factor": 4.0})
+    x.requires_grad_()
+    y, _ = ops().rotary(x, None, pos, tab, interleaved=True)
+    y.backward(dy)
+    with torch.no_grad():
+        z, _ = ops().rotary(x + u, None, pos, tab, interleaved=True)
+        lhs = (dy.double() * (z.double() - y.double())).sum()
+        rhs = (x.grad.double() * ((x + u) - x).double()).sum()
+        lim = 8 * 2.0 ** -24 * float((dy.abs().double() * (y.abs() + z.abs() + 1)).sum())
+    assert abs(float(lhs - rhs)) <= lim
+
+
+def test_rotary_gradient_captured():
+    """Forward and backward of a step in one graph, replayed with other values beside eager work."""
+    n, d = 40, 64
+    pos = torch.arange(n, device=DEV).int()
+    tab = ops().rotary_tables(64, d, 10000.0, DEV)
+    x = torch.zeros(n, 4, d, device=DEV, requires_grad=True)
+    dy = torch.zeros(n, 4, d, device=DEV)
+
+    def step():
+        y, _ = ops().rotary(x, None, pos, tab)
+        return torch.autograd.grad(y, x, dy)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dx = step()
+    for i in range(3):
+        dy.copy_(torch.randn(n, 4, d, generator=gen(40 + i), device=DEV))
+        pos.copy_((torch.arange(n, device=DEV) + i) % 64)
+        graph.replay()
+        want = ops().rotary(dy, None, pos, tab, backward=True)[0]
+        torch.cuda.synchronize()
+        assert torch.equal(dx, want), i

@@ -235,3 +235,29 @@ def test_division_by_a_multiply_is_exact():
             if 0 <= n < 2 ** 31:
                 s = ((n * m) >> 32) + n
                 assert s < 1 << 32 and s >> L == n // d, (n, d)
+
+
+def test_gradients_are_not_lost_silently():
+    """A call that records no gradient refuses tensors that want one, unless gradients are off."""
+    wants = lambda *s: torch.zeros(*s, dtype=BF, requires_grad=True)  # noqa: E731
+
+    def append(a):
+        return ops.paged_append(a["k"], a["v"], a["kc"], a["vc"], a["table"], a["q_start"], a["kv_len"], q=a["q"],
+                                q_out=a["q_out"])
+
+    def attend(a):
+        return ops.paged_attn(a["q"], a["kc"], a["vc"], a["table"], a["q_start"], a["kv_len"], 0.1)
+
+    cache = wants(5, 2, 16, 64)
+    calls = [(append, _cache(k=wants(3, 2, 64))), (append, _cache(v=wants(3, 2, 64))),
+             (append, _cache(q=wants(3, 4, 64))),
+             (attend, _cache(q=wants(3, 4, 64))), (attend, _cache(vc=cache)),
+             (lambda a: _rot(**a), dict(q=wants(3, 4, 64), out=(torch.zeros(3, 4, 64, dtype=BF),
+                                                                torch.zeros(3, 2, 64, dtype=BF)))),
+             (lambda a: _rot(**a), dict(tables=(torch.zeros(8, 32, requires_grad=True), torch.zeros(8, 32))))]
+    for f, a in calls:
+        with pytest.raises(ValueError, match="no gradient is recorded"):
+            f(a)
+        for off in (torch.no_grad(), torch.inference_mode()):
+            with off, pytest.raises(ValueError, match="device tensors"):
+                f(a)
