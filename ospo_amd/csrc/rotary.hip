@@ -329,7 +329,9 @@ extern "C" int ospo_paged_append(const void* k, long k_ts, long k_hs, const void
   if ((long)max_pages * page_size > 0x7fff0000L) return OSPO_ERR_SHAPE;
   if (rot_dim > 0 && n_pos < 1) return OSPO_ERR_SHAPE;
   if (n == 0 || n_seqs == 0) return OSPO_OK;
-  if (!k || !v || !k_cache || !v_cache || !block_table || !q_start || !kv_len) return OSPO_ERR_ARG;
+  if (!k || !v || !q_start || !kv_len) return OSPO_ERR_ARG;
+  // a cache without pages and a table without columns hold no address: no row is stored
+  if ((n_pages > 0 && (!k_cache || !v_cache)) || (max_pages > 0 && !block_table)) return OSPO_ERR_ARG;
   if (rot_dim > 0 && (!cos_tab || !sin_tab)) return OSPO_ERR_ARG;
   if (n_q_heads && (!q || !q_out)) return OSPO_ERR_ARG;
   a.cos_t = cos_tab, a.sin_t = sin_tab, a.n_pos = n_pos, a.sgn = 1.f, a.copy = 1;

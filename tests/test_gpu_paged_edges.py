@@ -172,3 +172,25 @@ def test_rotary_gradient_captured():
         want = ops().rotary(dy, None, pos, tab, backward=True)[0]
         torch.cuda.synchronize()
         assert torch.equal(dx, want), i
+
+
+# ------------------------------------------------------- caches without pages
+@pytest.mark.parametrize("pages,columns", [(0, 3), (4, 0), (0, 0)])
+def test_cache_without_pages(pages, columns):
+    """No row is stored, every query is turned, and a row of the attention sees nothing."""
+    n, hq, hk, d = 5, 4, 2, 64
+    g = gen(51)
+    q, k, v = (torch.randn(n, h, d, generator=g, device=DEV).to(BF) for h in (hq, hk, hk))
+    kc = torch.randn(pages, hk, 16, d, generator=g, device=DEV).to(BF)
+    vc = kc.clone()
+    table = torch.zeros(2, columns, dtype=torch.int32, device=DEV)
+    q_start = torch.tensor([0, 2, 5], dtype=torch.int32, device=DEV)
+    kv_len = torch.tensor([9, 3], dtype=torch.int32, device=DEV)
+    tab = ops().rotary_tables(16, d, 10000.0, DEV)
+    q_out = ops().paged_append(k, v, kc, vc, table, q_start, kv_len, q=q, rope=tab)
+    pos = torch.tensor([7, 8, 0, 1, 2], dtype=torch.int32, device=DEV)
+    assert torch.equal(q_out, ops().rotary(q, None, pos, tab)[0])
+    assert torch.equal(kc, vc)  # (as they were)
+    lse = torch.zeros(n, hq, device=DEV)
+    out = ops().paged_attn(q_out, kc, vc, table, q_start, kv_len, 0.1, lse=lse)
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all())
