@@ -1246,6 +1246,7 @@ struct Plan {
   int BM, KU;
   long pairs, items;  // upper bounds: (tile, head) pairs and items
   int slots, split;
+  bool sums;  // 64 sequences' (tile, head) pairs, counted with all rows each, fit 32 bits
   size_t o_off, ml_off, bytes;
 };
 
@@ -1281,7 +1282,9 @@ Plan make_plan(long rows, int S, int Hq, int Hk, int D, long most) {
   // 1000, 4000: 20 / 18, 37 / 21, 105 / 28; four chunks of 256 tokens (half of the slots) over 200, 1000, 1500, 4000:
   // 26 / 35, 42 / 45, 55 / 52, 112 / 86; four of 512 (all slots) over 0, 512, 1000: 26 / 33, 41 / 47, 56 / 62.
   const long bar = few ? 640 + 384 * p.pairs / p.slots : 256 + 2048 * p.pairs / p.slots;
-  p.split = most > bar && least < 4l * p.slots;
+  // (a q_start that descends may give every sequence all rows: not split where the device's sums of that could wrap)
+  p.split = most > bar && least < 4l * p.slots && least * S < (1l << 30);
+  p.sums = least < (1l << 25);
   p.items = !p.split ? p.pairs : p.pairs <= p.slots ? p.slots : p.pairs + 4l * p.slots;
   p.o_off = (size_t)(PLAN_HEAD + p.pairs * RECORD) * 4;  // bytes, a multiple of 16
   p.ml_off = p.o_off + (size_t)p.items * p.BM * D * 4;
@@ -1348,7 +1351,7 @@ extern "C" int ospo_paged_attn(const void* q, long q_ts, long q_hs, const void* 
   if (keys && (!aligned16(k_cache) || !aligned16(v_cache))) return OSPO_ERR_ALIGN;
   if (page_stride % 8 || head_stride % 8 || slot_stride % 8) return OSPO_ERR_ALIGN;
   const Plan p = make_plan(n, n_seqs, n_q_heads, n_kv_heads, head_dim, (long)page_size * max_pages);
-  if (p.items > 0x7fffffffL || p.pairs > 0x7fffffffL) return OSPO_ERR_SHAPE;
+  if (p.items > 0x7fffffffL || p.pairs > 0x7fffffffL || !p.sums) return OSPO_ERR_SHAPE;
   if (p.split && (!ws || ws_bytes < p.bytes)) return OSPO_ERR_ARG;
   if (p.split && !aligned16(ws)) return OSPO_ERR_ALIGN;
   PagedArgs a{};

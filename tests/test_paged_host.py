@@ -261,3 +261,17 @@ def test_gradients_are_not_lost_silently():
         for off in (torch.no_grad(), torch.inference_mode()):
             with off, pytest.raises(ValueError, match="device tensors"):
                 f(a)
+
+
+def test_sums_of_any_q_start_fit_32_bits():
+    """q_start is read on the device and may descend, so that every sequence has all rows.  Where the sums of row tiles
+    over all of them could pass 2^31 (and land on a count of records that nothing wrote), no keys are cut: no
+    workspace, no joining launch.  Where those of the 64 sequences of one scan could, the call is refused."""
+    ws = lambda n, S, hq, hk: _lib.query("ospo_paged_attn_ws_bytes", n, S, hq, hk, 128, 16, 4096)  # noqa: E731
+    for n, S, hk, cut in ((49136, 1 << 18, 1, True), (49136, 1 << 20, 1, False), (16, 1 << 19, 2048, False),
+                          (1, 1, 32, True), (4000, 1000, 8, True)):
+        bm = 16 if n <= 32 * S else 256
+        least = -(-n // bm) * hk
+        assert (least * S < 1 << 30) == cut
+        assert (ws(n, S, hk, hk) > 0) == cut, (n, S, hk)
+    assert c_attn(n=1 << 26, S=1 << 22, hq=32, hk=32) == 1
