@@ -13,6 +13,7 @@
 // (maximum, sum, O) in fp32 and a second launch joins them in chunk order: no atomics, the same bits each time.
 #include <math.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "paged.h"
@@ -44,6 +45,7 @@ struct PagedArgs {
   int qvec, ovec;  // q rows and o rows allow 16-byte access
   int slots;       // workgroups that run at once: what a split aims for
   int split;       // 0: every item is one chunk
+  int bar;         // keys are not cut where no sequence sees more of them than this
   long items, pairs;  // workgroups of the two launches: upper bounds
   int* plan;       // number of (tile, head) pairs, then from PLAN_HEAD on their records for the joining launch
   float* ws;       // partial O [item][BM][D]
@@ -111,13 +113,15 @@ template <int BM, int KU>
 __device__ __forceinline__ unsigned pick_chunk(const PagedArgs& a, int lane, const LaneSeq& first) {
   if (!a.split) return 0x7fffffff;
   float total = 0.f;
-  int base = 0, most = 1;
+  int base = 0, most = 1, longest = 0;
   for (int s0 = 0; s0 < a.S; s0 += 64) {
     const LaneSeq q = s0 ? lane_seq<BM, KU>(a, s0 + lane) : first;
     total += sum_f((float)q.tiles * (float)q.units);
     base += sum_i(q.tiles);
     most = max(most, max_i(q.tiles ? q.units : 0));
+    longest = max(longest, max_i(q.tiles ? max(q.q.kv - q.q.st, 0) : 0));
   }
+  if (longest <= a.bar) return 0x7fffffff;
   base = max(1, base * a.Hk);
   total *= (float)a.Hk;
   const float L = total / (float)a.slots;
@@ -1246,6 +1250,7 @@ struct Plan {
   int BM, KU;
   long pairs, items;  // upper bounds: (tile, head) pairs and items
   int slots, split;
+  long bar;   // keys that one sequence has to see before any are cut (on the device)
   bool sums;  // 64 sequences' (tile, head) pairs, counted with all rows each, fit 32 bits
   size_t o_off, ml_off, bytes;
 };
@@ -1281,8 +1286,15 @@ Plan make_plan(long rows, int S, int Hq, int Hk, int D, long most) {
   // token, 8 key/value heads of 128, 400, 700, 1000, 4000 keys 12 / 16, 16 / 16, 20 / 16, 60 / 15 us; 64 tokens over 200,
   // 1000, 4000: 20 / 18, 37 / 21, 105 / 28; four chunks of 256 tokens (half of the slots) over 200, 1000, 1500, 4000:
   // 26 / 35, 42 / 45, 55 / 52, 112 / 86; four of 512 (all slots) over 0, 512, 1000: 26 / 33, 41 / 47, 56 / 62.
+  // Those are calls, two launches against one.  The host knows only the table's width, and a captured step's table is as
+  // wide as its sequences may ever get: whether keys are cut then follows on the device from the longest sequence, by a bar
+  // of the kernels' times alone.  Uncut against cut, captured, a table of 200,000 keys: one token, 8 heads of keys and
+  // values, 256, 512, 1000 keys 11.8 / 11.4, 14.9 / 11.8, 22.7 / 11.6 us; 8 sequences of 32 heads 13.2 / 15.2, 19.5 / 20.5,
+  // 29.4 / 30.5; 64 tokens over 0, 256, 1000: 14.7 / 15.0, 20.7 / 18.5, 39.3 / 22.4; four chunks of 256 over 0, 512, 1000:
+  // 20.8 / 32.2, 33.0 / 39.3, 46.8 / 47.1.
   const long bar = few ? 640 + 384 * p.pairs / p.slots : 256 + 2048 * p.pairs / p.slots;
   // (a q_start that descends may give every sequence all rows: not split where the device's sums of that could wrap)
+  p.bar = few ? std::min(bar, 256 + 1536 * p.pairs / p.slots) : 96 + 1900 * p.pairs / p.slots;
   p.split = most > bar && least < 4l * p.slots && least * S < (1l << 30);
   p.sums = least < (1l << 25);
   p.items = !p.split ? p.pairs : p.pairs <= p.slots ? p.slots : p.pairs + 4l * p.slots;
@@ -1367,7 +1379,7 @@ extern "C" int ospo_paged_attn(const void* q, long q_ts, long q_hs, const void* 
   a.causal = causal;
   a.qvec = aligned16(q) && q_ts % 8 == 0 && q_hs % 8 == 0;
   a.ovec = aligned16(out) && o_ts % 8 == 0 && o_hs % 8 == 0;
-  a.slots = p.slots, a.split = p.split, a.items = p.items, a.pairs = p.pairs;
+  a.slots = p.slots, a.split = p.split, a.bar = (int)std::min(p.bar, 0x7fffffffL), a.items = p.items, a.pairs = p.pairs;
   a.plan = (int*)ws, a.ws = (float*)((char*)ws + p.o_off), a.ml = (float*)((char*)ws + p.ml_off);
   if (dtype == DT_BF16) {
     switch (head_dim) {

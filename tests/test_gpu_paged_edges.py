@@ -194,3 +194,21 @@ def test_cache_without_pages(pages, columns):
     lse = torch.zeros(n, hq, device=DEV)
     out = ops().paged_attn(q_out, kc, vc, table, q_start, kv_len, 0.1, lse=lse)
     assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+
+
+# ---------------------------------------------------------- cutting the keys
+@pytest.mark.parametrize("new,total,hq,hk", [
+    ([1] * 32, [24 + 19 * i for i in range(32)], 32, 32),  # a sampling step: more tiles than places, nothing to cut
+    ([200, 90, 150], [200, 300, 150], 8, 8),               # many rows, too short to cut
+    ([1, 1], [5000, 300], 8, 2),                           # long enough
+    ([200, 90, 1], [200, 6000, 150], 8, 4)])
+@pytest.mark.parametrize("d,dtype", [(64, HF), (128, BF)])
+def test_a_wider_table_cuts_no_more(new, total, hq, hk, d, dtype):
+    """A table with room for longer sequences (a captured step's) gives the same bits: its keys are cut by the lengths
+    on the device, where some sequence is long enough."""
+    s = R.build(new, total, hq=hq, hk=hk, d=d, page=16, dtype=dtype, seed=61, device=DEV)
+    want, wl = check(s, d ** -0.5)
+    wide = torch.zeros(len(new), 2048, dtype=torch.int32, device=DEV)
+    wide[:, : s["table"].shape[1]] = s["table"]
+    got, gl = check(dict(s, table=wide), d ** -0.5)
+    assert torch.equal(got, want) and torch.equal(gl, wl)
