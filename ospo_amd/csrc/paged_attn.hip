@@ -48,8 +48,9 @@ struct PagedArgs {
   int bar;         // keys are not cut where no sequence sees more of them than this
   long items, pairs;  // workgroups of the two launches: upper bounds
   int* plan;       // number of (tile, head) pairs, then from PLAN_HEAD on their records for the joining launch
-  float* ws;       // partial O [item][BM][D]
-  float* ml;       // (m, l) [item][BM][2]
+  float* ws;       // partial O [row of a cut item][D]
+  float* ml;       // (m, l) [row of a cut item][2]
+  int cap;         // rows that both hold
 };
 
 // ---------------------------------------------------------------- items
@@ -110,8 +111,7 @@ __device__ __forceinline__ LaneSeq lane_seq(const PagedArgs& a, int s) {
 // of L, the smallest chunk that might do, and of the smaller of two that do (every tile cut as the longest may be;
 // the work over the slots that the tiles leave), the first of four steps from one to the other that fits.
 template <int BM, int KU>
-__device__ __forceinline__ unsigned pick_chunk(const PagedArgs& a, int lane, const LaneSeq& first) {
-  if (!a.split) return 0x7fffffff;
+__device__ __forceinline__ unsigned even_chunk(const PagedArgs& a, int lane, const LaneSeq& first) {
   float total = 0.f;
   int base = 0, most = 1, longest = 0;
   for (int s0 = 0; s0 < a.S; s0 += 64) {
@@ -143,11 +143,30 @@ __device__ __forceinline__ unsigned pick_chunk(const PagedArgs& a, int lane, con
   }
   return (unsigned)hi;
 }
+__device__ __forceinline__ int chunks_of(const LaneSeq& q, unsigned C) { return (int)(((unsigned)q.units - 1) / C) + 1; }
+// That chunk, larger where the partial results of the sequences that it cuts would not fit the workspace.  (One that cuts
+// nothing needs none.)
+template <int BM, int KU>
+__device__ __forceinline__ unsigned pick_chunk(const PagedArgs& a, int lane, const LaneSeq& first) {
+  if (!a.split) return 0x7fffffff;
+  unsigned C = even_chunk<BM, KU>(a, lane, first);
+  for (;;) {
+    float need = 0.f;  // (the sum is exact up to 2^24, more than the workspace holds)
+    for (int s0 = 0; s0 < a.S; s0 += 64) {
+      const LaneSeq q = s0 ? lane_seq<BM, KU>(a, s0 + lane) : first;
+      const int nch = chunks_of(q, C);
+      need += sum_f(nch > 1 ? (float)q.q.n * (float)a.g.d * (float)nch : 0.f);
+    }
+    need *= (float)a.Hk;
+    if (need <= (float)a.cap) return C;
+    C = (unsigned)fminf(ceilf((float)C * fmaxf(need / (float)a.cap, 1.125f)), 2e9f);
+  }
+}
 
 struct Item {
   Seq q;
   int seq, tile, head, chunk, nch, cs, u0, units;
-  int step;  // the item indices of a (tile, head)'s chunks are this far apart
+  int slot;  // partial results: of the tile's first row
   int pair;  // number of the (tile, head)
 };
 // Order of a sequence's items: heads fastest over the XCDs (hb = largest power of two <= 8 that divides Hk, so a
@@ -157,13 +176,14 @@ template <int BM, int KU>
 __device__ __forceinline__ bool find_item(const PagedArgs& a, int id, int lane, Item& it) {
   const LaneSeq lead = lane_seq<BM, KU>(a, lane);
   const unsigned C = pick_chunk<BM, KU>(a, lane, lead);
-  int before = 0, pairs = 0;
+  int before = 0, pairs = 0, slots = 0;
   bool got = false;
   for (int s0 = 0; s0 < a.S; s0 += 64) {
     const LaneSeq q = s0 ? lane_seq<BM, KU>(a, s0 + lane) : lead;
-    const int nch = (int)(((unsigned)q.units - 1) / C) + 1;
+    const int nch = chunks_of(q, C);
     const int own = q.tiles * a.Hk, mine = own * nch;
-    const int upto = scan_add(mine), pupto = scan_add(own);
+    const int cut = nch > 1 ? q.q.n * (int)a.g.d * nch * a.Hk : 0;
+    const int upto = scan_add(mine), pupto = scan_add(own), cupto = scan_add(cut);
     const unsigned long long b = __ballot(id - before < upto);
     if (b && !got) {
       const int w = __ffsll(b) - 1;
@@ -181,13 +201,14 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int id, int lane, 
       it.chunk = (int)(x - tx * it.nch);
       it.cs = (int)(((unsigned)it.units + it.nch - 1) / it.nch);
       it.u0 = it.q.st / KU;
-      it.step = hb;
+      it.slot = slots + lane_of(cupto - cut, w) + (it.head * it.nch + it.chunk) * it.q.n * (int)a.g.d + it.tile * BM;
       it.pair = pairs + lane_of(pupto - own, w) + (int)(((hh * tiles + tx) << sh) + (at & (hb - 1)));
       got = true;
       if (id > 0) return true;
     }
     before += lane_of(upto, 63);
     pairs += lane_of(pupto, 63);
+    slots += lane_of(cupto, 63);
   }
   // (more than the launches' bounds only where q_start descends: nothing is joined then)
   if (id == 0 && a.split && threadIdx.x == 0) a.plan[0] = before <= a.items && pairs <= a.pairs ? pairs : 0;
@@ -200,7 +221,8 @@ __device__ __forceinline__ int tile_end(const PagedArgs& a, const Item& it, int 
   return max(0, it.q.kv - it.q.n + fdiv(last, a.g) + 1);
 }
 
-// What the joining launch needs to know of a (tile, head): how many chunks to join (0: none), its first item.
+// What the joining launch needs to know of a (tile, head): how many chunks to join (0: none), where the first row's partial
+// results lie, and how far on those of the next chunk.
 struct Record {
   int chunks, first, step, q0, head, row0, rows;
 };
@@ -210,7 +232,7 @@ __device__ __forceinline__ void note(const PagedArgs& a, const Item& it, int end
   if (!a.split || it.chunk > 0 || threadIdx.x) return;
   const int left = min(end, (it.u0 + it.units) * KU) - it.u0 * KU;
   const int n = left > 0 ? ((left + KU - 1) / KU + it.cs - 1) / it.cs : 1;  // chunks that have keys (one writes if none has)
-  Record r{it.nch > 1 ? n : 0, (int)blockIdx.x, it.step, it.q.q0, it.head, it.tile * BM,
+  Record r{it.nch > 1 ? n : 0, it.slot, it.q.n * (int)a.g.d, it.q.q0, it.head, it.tile * BM,
            min(BM, it.q.n * (int)a.g.d - it.tile * BM)};
   if (it.pair < a.pairs) *reinterpret_cast<Record*>(a.plan + PLAN_HEAD + (long)it.pair * RECORD) = r;
 }
@@ -793,7 +815,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
       }
     }
     if (part) {
-      const long slot = (long)blockIdx.x * BM + (r - R0);
+      const long slot = it.slot + (r - R0);
       if (r < R) {
         if (hi == 0) *reinterpret_cast<f32x2*>(a.ml + slot * 2) = f32x2{m[b], L};
         float* to = a.ws + slot * D + 4 * hi;
@@ -1193,7 +1215,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_per_cu(
       for (int e = 0; e < 4; ++e) x[e] += y[e] * w;
     }
     if (part) {
-      const long slot = (long)blockIdx.x * BM + lr;
+      const long slot = it.slot + lr;
       *reinterpret_cast<f32x4*>(a.ws + slot * D + d0) = f32x4{x[0], x[1], x[2], x[3]};
       if (d0 == 0) *reinterpret_cast<f32x2*>(a.ml + slot * 2) = f32x2{M, L};
     } else {
@@ -1212,9 +1234,9 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a) {
   if (it.chunks <= 0 || r0 >= it.rows) return;
   constexpr int TPR = D / 4, RPB = 256 / TPR, AT = 8;  // chunks on their way at once
   const int d0 = (threadIdx.x % TPR) * 4;
-  const long ds = (long)it.step * BM;
+  const long ds = it.step;
   for (int lr = r0 + threadIdx.x / TPR; lr < min(r0 + ROWS, it.rows); lr += RPB) {
-    const long s0 = (long)it.first * BM + lr;
+    const long s0 = it.first + lr;
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
     float M = NONE, L = 0.f;
     for (int c0 = 0; c0 < it.chunks; c0 += AT) {
@@ -1249,6 +1271,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedArgs a) {
 struct Plan {
   int BM, KU;
   long pairs, items;  // upper bounds: (tile, head) pairs and items
+  long cap;           // rows of partial results
   int slots, split;
   long bar;   // keys that one sequence has to see before any are cut (on the device)
   bool sums;  // 64 sequences' (tile, head) pairs, counted with all rows each, fit 32 bits
@@ -1299,8 +1322,12 @@ Plan make_plan(long rows, int S, int Hq, int Hk, int D, long most) {
   p.sums = least < (1l << 25);
   p.items = !p.split ? p.pairs : p.pairs <= p.slots ? p.slots : p.pairs + 4l * p.slots;
   p.o_off = (size_t)(PLAN_HEAD + p.pairs * RECORD) * 4;  // bytes, a multiple of 16
-  p.ml_off = p.o_off + (size_t)p.items * p.BM * D * 4;
-  p.bytes = p.split ? p.ml_off + (size_t)p.items * p.BM * 2 * 4 : 0;
+  // Partial results: a tile's rows for every place of the launch, or all rows over all key blocks, where that is less.
+  // Filling the places once takes no more.  Evening out several rounds may: four tiles' then of few rows, and beyond that
+  // larger chunks (pick_chunk).  34 MB at most.
+  p.cap = (long)std::min((double)p.slots * p.BM * (few && p.pairs > p.slots ? 4 : 1), (double)rows * g * Hk * ((most + p.KU - 1) / p.KU));
+  p.ml_off = p.o_off + (size_t)p.cap * D * 4;
+  p.bytes = p.split ? p.ml_off + (size_t)p.cap * 2 * 4 : 0;
   return p;
 }
 
@@ -1380,6 +1407,7 @@ extern "C" int ospo_paged_attn(const void* q, long q_ts, long q_hs, const void* 
   a.qvec = aligned16(q) && q_ts % 8 == 0 && q_hs % 8 == 0;
   a.ovec = aligned16(out) && o_ts % 8 == 0 && o_hs % 8 == 0;
   a.slots = p.slots, a.split = p.split, a.bar = (int)std::min(p.bar, 0x7fffffffL), a.items = p.items, a.pairs = p.pairs;
+  a.cap = (int)p.cap;
   a.plan = (int*)ws, a.ws = (float*)((char*)ws + p.o_off), a.ml = (float*)((char*)ws + p.ml_off);
   if (dtype == DT_BF16) {
     switch (head_dim) {

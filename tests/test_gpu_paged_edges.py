@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from tests import paged_ref as R
+from tests.paged_cases import WAYS, WINDOWS
 from tests.test_gpu_paged import check, gen
 
 pytestmark = pytest.mark.gpu
@@ -212,3 +213,98 @@ def test_a_wider_table_cuts_no_more(new, total, hq, hk, d, dtype):
     wide[:, : s["table"].shape[1]] = s["table"]
     got, gl = check(dict(s, table=wide), d ** -0.5)
     assert torch.equal(got, want) and torch.equal(gl, wl)
+
+
+def spot_check(c, d, dtype, seed):
+    """A batch against the plain form, heads and sequences thinned where the batch is large (each head and each sequence is
+    an item of its own): the first and last sequences and every fifth, the first, middle and last key/value heads."""
+    new, kv, hq, hk, page = c["new"], c["kv"], c["hq"], c["hk"], c["page"]
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    pages = [-(-t // page) for t in kv]
+    order = torch.randperm(sum(pages) + 2, generator=g, device=DEV)
+    kc = torch.randn(order.numel(), hk, page, d, generator=g, device=DEV, dtype=dtype)
+    vc = torch.randn(order.numel(), hk, page, d, generator=g, device=DEV, dtype=dtype)
+    table = torch.zeros(len(new), c["columns"], dtype=torch.int32, device=DEV)
+    at = 0
+    for b, p in enumerate(pages):
+        table[b, :p] = order[at: at + p].int()
+        if kv[b] % page:  # slots behind the end
+            kc[order[at + p - 1], :, kv[b] % page:] = math.nan
+            vc[order[at + p - 1], :, kv[b] % page:] = math.nan
+        at += p
+    q = torch.randn(sum(new), hq, d, generator=g, device=DEV, dtype=dtype)
+    q_start = torch.tensor([sum(new[:i]) for i in range(len(new) + 1)], dtype=torch.int32, device=DEV)
+    kv_len = torch.tensor(kv, dtype=torch.int32, device=DEV)
+    lse = torch.full((sum(new), hq), 3.0, device=DEV)
+    out = ops().paged_attn(q, kc, vc, table, q_start, kv_len, d ** -0.5, lse=lse)
+    again = ops().paged_attn(q, kc, vc, table, q_start, kv_len, d ** -0.5)
+    assert torch.equal(out, again)
+    seqs = sorted({0, len(new) - 1, *range(0, len(new), 5)})
+    for h in sorted({0, hk // 2, hk - 1}):
+        heads = slice(h * (hq // hk), (h + 1) * (hq // hk))
+        for b in seqs:
+            rows = slice(int(q_start[b]), int(q_start[b + 1]))
+            one = torch.tensor([0, new[b]], dtype=torch.int32)
+            ref, rl, tol, ltol, _ = R.attend(q[rows, heads], kc[:, h: h + 1], vc[:, h: h + 1], table[b: b + 1], one,
+                                             kv_len[b: b + 1], d ** -0.5)
+            ok, worst = R.within(out[rows, heads], ref, tol, dtype)
+            assert ok, (b, h, worst)
+            assert bool(((lse[rows, heads].double() - rl).abs() <= ltol).all()), (b, h)
+    assert bool(out.isfinite().all()) and bool(lse.isfinite().all())
+
+
+@pytest.mark.parametrize("name,d", [(n, d) for n in sorted(WAYS) for d in WAYS[n]["d"]])
+def test_every_way_of_the_rule(name, d):
+    spot_check(WAYS[name], d, HF if d == 64 else BF, 71)
+
+
+@pytest.mark.parametrize("name", sorted(WINDOWS))
+def test_windows_of_page_numbers(name):
+    spot_check(WINDOWS[name], WINDOWS[name]["d"], BF, 72)
+
+
+# ------------------------------------------------------------ many rows, more
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("new,total,at", [(130, 700, 3), (130, 700, 400), (130, 700, 640), (2, 700, 300)])
+@pytest.mark.parametrize("d,dtype", [(64, HF), (128, BF), (256, BF)])
+def test_values_that_are_not_finite_while_maxima_rise(value, new, total, at, d, dtype):
+    """Keys lengthen along the sequence, so that maxima rise by many powers of two from tile to tile, and one visible value
+    is not finite.  Its probability in 32 bits is zero for most later rows, where a product of zero and infinity may be
+    NaN: its column of its head is infinite or NaN, all else is as without it."""
+    s = R.build([new], [total], hq=4, hk=2, d=d, page=16, dtype=dtype, seed=81, device=DEV)
+    j = torch.arange(total, device=DEV)
+    p = s["table"][0].long()[j // 16]
+    f = (1 + j.float() / 8).clamp(max=90.0)[:, None, None]
+    s["kc"][p, :, j % 16] = (s["kc"][p, :, j % 16].float() * f).to(dtype)
+    check(s, d ** -0.5)
+    args = (s["q"], s["kc"], s["vc"], s["table"], s["q_start"], s["kv_len"], d ** -0.5)
+    lse = torch.zeros(new, 4, device=DEV)
+    clean = ops().paged_attn(*args)
+    s["vc"][p[at], 1, at % 16, d - 3] = value
+    got = ops().paged_attn(*args, lse=lse)
+    first = max(0, at - (total - new))  # rows from here on see it
+    assert bool((~got[first:, 2:, d - 3].isfinite()).all())
+    got[first:, 2:, d - 3] = clean[first:, 2:, d - 3]
+    assert torch.allclose(got.float(), clean.float(), rtol=2.0 ** -7, atol=2.0 ** -9)
+    assert bool(lse.isfinite().all())
+
+
+@pytest.mark.parametrize("new,total", [([70, 3], [200, 130]), ([1, 2], [200, 30])])
+def test_slots_far_apart(new, total):
+    """Slots 2^26 elements apart (16 of them are 2 GiB), where the many-row kernel's 32-bit byte offsets end."""
+    hk, d, page, stride = 2, 128, 16, 1 << 26
+    s = R.build(new, total, hq=4, hk=hk, d=d, page=page, dtype=BF, seed=91, device=DEV)
+    want, wl = check(s, d ** -0.5)
+    far = {}
+    for name in ("kc", "vc"):
+        c = s[name]
+        flat = torch.empty(stride * (page - 1) + c.shape[0] * hk * d, dtype=BF, device=DEV)
+        far[name] = flat.as_strided(c.shape, (hk * d, d, stride, 1))
+        far[name].copy_(c)
+    got, gl = check(dict(s, **far), d ** -0.5)
+    assert torch.equal(got, want) and torch.equal(gl, wl)
+    g = gen(92)
+    k, v = (torch.randn(sum(new), hk, d, generator=g, device=DEV).to(BF) for _ in range(2))
+    ops().paged_append(k, v, s["kc"], s["vc"], s["table"], s["q_start"], s["kv_len"])
+    ops().paged_append(k, v, far["kc"], far["vc"], s["table"], s["q_start"], s["kv_len"])
+    assert torch.equal(far["kc"], s["kc"]) and torch.equal(far["vc"], s["vc"])

@@ -275,3 +275,23 @@ def test_sums_of_any_q_start_fit_32_bits():
         assert (least * S < 1 << 30) == cut
         assert (ws(n, S, hk, hk) > 0) == cut, (n, S, hk)
     assert c_attn(n=1 << 26, S=1 << 22, hq=32, hk=32) == 1
+
+
+@pytest.mark.parametrize("n,S,hq,hk,d,page,columns", [
+    (575, 64, 32, 8, 128, 64, 128),        # a chunk of 512 tokens and 63 single ones
+    (3300, 100, 32, 32, 128, 16, 2048), (8001, 1000, 32, 8, 128, 16, 8192), (8, 8, 32, 8, 128, 64, 512),
+    (512, 1, 32, 8, 128, 64, 4096), (2048, 64, 32, 8, 256, 64, 4096), (64, 2048, 32, 32, 64, 16, 2048)])
+def test_workspace_of_the_attention_is_bounded(n, S, hq, hk, d, page, columns):
+    """Partial results of a tile's rows (few rows in more tiles than places: of four) for each of a launch's places,
+    however many sequences there are, and 32 bytes for each (tile, head)."""
+    b = _lib.query("ospo_paged_attn_ws_bytes", n, S, hq, hk, d, page, columns)
+    g = hq // hk
+    bm = 16 if n * g <= 32 * S else 128 if d > 128 else 256
+    pairs = min(n * g // bm + S, n * -(-g // bm)) * hk
+    places = 256 * ({64: 4, 128: 3, 256: 2}[d] if bm == 16 else 1)
+    rows = min(places * bm * (4 if bm == 16 and pairs > places else 1),
+               n * hq * -(-page * columns // (128 if bm == 16 else 64)))
+    assert b == 32 + 32 * pairs + rows * (4 * d + 8)
+    assert b < 40e6
+    one = _lib.query("ospo_paged_attn_ws_bytes", 1, 1, 32, 8, d, page, columns)
+    assert 0 < one < 14e6
