@@ -535,13 +535,14 @@ int ospo_decode_attn_o(const void* q, int ldq, const void* k_cache, const void* 
 
 /* ------------------------------------------------------------ paged cache ---
  * Serving over a cache of pages: unlike lengths side by side, grouped heads, long contexts.  bf16 (dtype 0) or fp16
- * (dtype 1), the rotation also fp32 (dtype 2).  Strides are in ELEMENTS; the last dimension is contiguous.
+ * (dtype 1); rotation and append also fp32 (dtype 2), which the attention does not read.  At most 4096 heads.  Strides are
+ * in ELEMENTS; the last dimension is contiguous.
  *
  * A batch is ragged: the rows (new tokens) of sequence s are q_start[s] .. q_start[s + 1] - 1 (int32 [n_seqs + 1],
  * not descending), kv_len[s] (int32) is its length WITH them, so row r sits at position
  * kv_len[s] - q_start[s + 1] + r.  Position p lives in page block_table[s][p / page_size] (int32
- * [n_seqs][max_pages]), slot p % page_size; page_size >= 1 is any number, max_pages * page_size < 2^31.  A cache
- * tensor is [n_pages][kv heads][page_size][head_dim] by page_stride, head_stride and slot_stride.  All of these
+ * [n_seqs][max_pages]), slot p % page_size; page_size >= 1 is any number, max_pages * page_size <= 2^31 - 2^16.
+ * A cache tensor is [n_pages][kv heads][page_size][head_dim] by page_stride, head_stride and slot_stride.  All of these
  * are read on the device: a captured call follows their values at each replay.  Values outside their range cannot
  * fault: row numbers and lengths are clamped to the buffers, a page outside [0, n_pages) is not written by the
  * append and read as the nearest page by the attention.  Rows of no sequence are left as they were.

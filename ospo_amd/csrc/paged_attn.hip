@@ -241,8 +241,7 @@ __device__ __forceinline__ void note(const PagedArgs& a, const Item& it, int end
 // mma: a product as the compiler sees it.  acc: one into accumulators that stay in the matrix unit's own registers (the
 // compiler moves some of O to vector registers and back around its products).  It knows nothing of the waits that
 // such a product needs: two states behind the vector unit's last write to an operand, which the block brings along,
-// and settle() before anything but another product reads the accumulators.
-__device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 7" ::: "memory"); }
+// and the kernel's settle before anything but another product reads the accumulators.
 //
 // A probability is held as exp2(x - m) in the cache's type, m = the row's largest x less FEW or MANY (few and many rows).
 // bf16 has fp32's exponents and needs no such offset.  fp16's last normal number is 2^-14 and its largest is 65504:
@@ -282,28 +281,13 @@ struct Frag<f16> {
   }
 };
 
-// A fragment of values as finite numbers (others as zeros), and where +infinity and -infinity (NaN: both) stand
+// 8 values with zeros for those that are not finite
 template <typename T>
-__device__ __forceinline__ void split_values(const i16x8& v, typename Frag<T>::v8& fin, typename Frag<T>::v8& up,
-                                             typename Frag<T>::v8& dn) {
+__device__ __forceinline__ i16x8 finite(i16x8 v) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const short e = v[i];  // (a copy: a bit cast of the vector's element itself takes element 0)
-    const unsigned bits = (unsigned short)e;
-    const bool odd = (bits & Frag<T>::EXP) == Frag<T>::EXP, nan = odd && (bits & Frag<T>::MAN);
-    fin[i] = odd ? (T)0.f : __builtin_bit_cast(T, e);
-    up[i] = nan || (odd && !(bits & 0x8000)) ? (T)1.f : (T)0.f;
-    dn[i] = nan || (odd && (bits & 0x8000)) ? (T)1.f : (T)0.f;
-  }
-}
-
-// LDS images are [key][D] with the 16-byte chunks of a row swizzled so that both the row reads of K (32 rows, one
-// chunk) and the transposed reads of V (4 rows x 4 chunks) meet every bank once: 256-byte rows rotate by
-// 4 (r & 3) + ((r >> 2) & 3) over 16 chunks, 128-byte rows (two share the banks) by 4 ((r >> 1) & 1) + ((r >> 2) & 3)
-// over 8.
-template <int D>
-__device__ __forceinline__ int swz(int r) {
-  return D >= 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+  for (int i = 0; i < 8; ++i)
+    if (((unsigned short)v[i] & Frag<T>::EXP) == Frag<T>::EXP) v[i] = 0;
+  return v;
 }
 
 // 16 bytes a lane from global memory to LDS (wave-uniform destination + 16 lane), without registers
@@ -615,9 +599,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) voi
 #pragma nounroll
     for (int p = 0; p < NL; ++p) {
       i16x8* x = reinterpret_cast<i16x8*>(vl + (4 * p + wave) * 1024 + lane * 16);
-      v8 fin, isup, isdn;
-      split_values<T>(*x, fin, isup, isdn);
-      *x = __builtin_bit_cast(i16x8, fin);
+      *x = finite<T>(*x);
     }
     sync_lds();
   };
@@ -1097,9 +1079,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(few_per_cu(
 #pragma nounroll
     for (int p = 0; p < 2 * KS; ++p) {
       i16x8* x = reinterpret_cast<i16x8*>(vl + p * 1024 + lane * 16);
-      v8 fin, up, dn;
-      split_values<T>(*x, fin, up, dn);
-      *x = __builtin_bit_cast(i16x8, fin);
+      *x = finite<T>(*x);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   };
