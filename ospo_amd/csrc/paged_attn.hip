@@ -359,7 +359,7 @@ constexpr int pitch_of(int D) { return D + 4; }  // floats of a staged output ro
 // which both types hold; sums stay in fp32.  (O is scaled where it is: put aside in memory and added up at the end, fp16's
 // chunks of up to 257 tokens over up to 5000 keys, a few of whose rows grow by 2^7, took 42 us instead of 21.)
 //
-// Measured: whole prompts of 3.5k to 4k tokens, 32 heads over 8 of 128, at 957 TFLOP/s (494 us for four).  A tile of 64
+// Measured: whole prompts of 3.5k to 4k tokens, 32 heads over 8 of 128, at 945 TFLOP/s (500 us for four).  A tile of 64
 // keys takes 3600 cycles, 2048 of them products; the matrix unit is busy for 54 % of all cycles.  32 instructions less a
 // tile (of 580) change nothing, no exponentials at all would gain 7 %, fragments read 2 or 4 slots ahead the same time.
 // The start of an item (lengths, page numbers, first keys: three round trips to memory, one behind the other) and its end
@@ -1271,9 +1271,11 @@ int device_cus() {
 }
 
 // At most 32 rows for each sequence and key/value head on average: the kernel for few rows.  Otherwise the one for many
-// (256-row tiles; 128 with 256-wide heads, whose O fills the registers at 32 rows a wave).  32 heads over 8 of 128, few
-// against many: 8 sequences of 4000 keys with 16, 32, 64 rows 31 / 38, 42 / 38, 67 / 40 us; 64 of 1000 keys 48 / 92,
-// 65 / 98, 122 / 109 us.
+// (256-row tiles; 128 with 256-wide heads, whose O fills the registers at 32 rows a wave).  Few against many, captured:
+// 32 heads over 8 of 128, 8 sequences of 4000 keys with 16, 32, 64 rows 33 / 42, 44 / 42, 68 / 44 us; 64 of 1000 keys 47 / 72,
+// 66 / 73, 124 / 77; 32 over 32, 8 of 4000 103 / 146, 128 / 153, 249 / 157; 16 over 4 of 64, 64 of 1000 20 / 27, 26 / 27,
+// 35 / 28.  It is one choice for the whole batch: a prompt beside enough single tokens, or in a batch whose other places are
+// empty, takes the kernel for few rows (4096 tokens of 32 heads in 256 places: 945 us, 206 alone).
 Plan make_plan(long rows, int S, int Hq, int Hk, int D, long most) {
   Plan p;
   const long g = Hq / Hk;
@@ -1285,19 +1287,20 @@ Plan make_plan(long rows, int S, int Hq, int Hk, int D, long most) {
   p.slots = device_cus() * (few ? few_per_cu(D) : 1);
   const long least = (rows * g + p.BM - 1) / p.BM * Hk;
   // Splitting costs the partial results' way through memory and a second launch.  It pays from more keys on the less room
-  // the tiles leave for chunks, and not where there are tiles enough for four rounds.  Not split against split: one
-  // token, 8 key/value heads of 128, 400, 700, 1000, 4000 keys 12 / 16, 16 / 16, 20 / 16, 60 / 15 us; 64 tokens over 200,
-  // 1000, 4000: 20 / 18, 37 / 21, 105 / 28; four chunks of 256 tokens (half of the slots) over 200, 1000, 1500, 4000:
-  // 26 / 35, 42 / 45, 55 / 52, 112 / 86; four of 512 (all slots) over 0, 512, 1000: 26 / 33, 41 / 47, 56 / 62.
+  // the tiles leave for chunks, and not where there are tiles enough for four rounds.  Whole against cut: one token, 32
+  // heads over 8 of 128, 400, 700, 1000, 4000 keys 12 / 17, 16 / 17, 20 / 17, 59 / 17 us; 8 times one token, 32 over 32,
+  // 400, 1000, 2000: 15 / 19, 26 / 30, 46 / 49; 64 tokens over 200, 1000, 4000: 19 / 19, 36 / 22, 105 / 28; four chunks of
+  // 256 tokens (half of the slots) over 200, 1000, 1500, 4000: 25 / 36, 42 / 46, 54 / 53, 111 / 87; four of 512 (all slots)
+  // over 0, 512, 1000, 4000: 24 / 33, 38 / 46, 54 / 62, 139 / 147 (equal lengths, where there is nothing to even out).
   // Those are calls, two launches against one.  The host knows only the table's width, and a captured step's table is as
   // wide as its sequences may ever get: whether keys are cut then follows on the device from the longest sequence, by a bar
-  // of the kernels' times alone.  Uncut against cut, captured, a table of 200,000 keys: one token, 8 heads of keys and
-  // values, 256, 512, 1000 keys 11.8 / 11.4, 14.9 / 11.8, 22.7 / 11.6 us; 8 sequences of 32 heads 13.2 / 15.2, 19.5 / 20.5,
-  // 29.4 / 30.5; 64 tokens over 0, 256, 1000: 14.7 / 15.0, 20.7 / 18.5, 39.3 / 22.4; four chunks of 256 over 0, 512, 1000:
-  // 20.8 / 32.2, 33.0 / 39.3, 46.8 / 47.1.
+  // of the kernels' times alone.  Whole against cut, captured, a table of 200,000 keys: one token, 32 heads over 8, 256,
+  // 512, 1000 keys 12.1 / 11.8, 15.0 / 12.1, 22.8 / 12.4 us; 8 times one token, 32 over 32, 13.3 / 15.7, 19.0 / 20.8,
+  // 29.3 / 30.7; 64 tokens over 0, 256, 1000: 14.4 / 15.1, 20.8 / 18.6, 39.5 / 22.0; four chunks of 256 over 0, 512, 1000:
+  // 21 / 32, 34 / 40, 48 / 48.
   const long bar = few ? 640 + 384 * p.pairs / p.slots : 256 + 2048 * p.pairs / p.slots;
-  // (a q_start that descends may give every sequence all rows: not split where the device's sums of that could wrap)
   p.bar = few ? std::min(bar, 256 + 1536 * p.pairs / p.slots) : 96 + 1900 * p.pairs / p.slots;
+  // (a q_start that descends may give every sequence all rows: not split where the device's sums of that could wrap)
   p.split = most > bar && least < 4l * p.slots && least * S < (1l << 30);
   p.sums = least < (1l << 25);
   p.items = !p.split ? p.pairs : p.pairs <= p.slots ? p.slots : p.pairs + 4l * p.slots;
@@ -1305,7 +1308,8 @@ Plan make_plan(long rows, int S, int Hq, int Hk, int D, long most) {
   // Partial results: a tile's rows for every place of the launch, or all rows over all key blocks, where that is less.
   // Filling the places once takes no more.  Evening out several rounds may: four tiles' then of few rows, and beyond that
   // larger chunks (pick_chunk).  34 MB at most.
-  p.cap = (long)std::min((double)p.slots * p.BM * (few && p.pairs > p.slots ? 4 : 1), (double)rows * g * Hk * ((most + p.KU - 1) / p.KU));
+  p.cap = (long)std::min((double)p.slots * p.BM * (few && p.pairs > p.slots ? 4 : 1),
+                         (double)rows * g * Hk * ((most + p.KU - 1) / p.KU));
   p.ml_off = p.o_off + (size_t)p.cap * D * 4;
   p.bytes = p.split ? p.ml_off + (size_t)p.cap * 2 * 4 : 0;
   return p;

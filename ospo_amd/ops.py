@@ -927,8 +927,9 @@ def rotary_tables(n_pos: int, rot_dim: int, theta: float, device, scaling: Optio
       {"type": "linear", "factor": s}: f_i / s;
       {"type": "ntk", "factor": s}: theta * s^(rot_dim / (rot_dim - 2)), so that the slowest pair turns s times slower;
       {"type": "yarn", "factor": s, "original": L, "beta_fast": 32, "beta_slow": 1, "magnitude": 0.1 ln s + 1}: pairs
-        that turn beta_fast times or more within L keep f_i, those below beta_slow get f_i / s, a linear ramp in
-        between (YaRN, Peng et al. 2023); both tables times the magnitude."""
+        that turn beta_fast times or more within L keep f_i, those below beta_slow get f_i / s, a linear ramp of the
+        turns in between (YaRN, Peng et al. 2023); both tables times the magnitude.  A model tuned with a ramp over the
+        pair's index between two rounded bounds needs tables of its own."""
     if n_pos < 1 or rot_dim < 2 or rot_dim % 2 or not theta > 0:
         raise ValueError(f"rotary_tables: n_pos {n_pos}, rot_dim {rot_dim}, theta {theta}")
     kind, s, mag = None, 1.0, 1.0
